@@ -424,6 +424,121 @@ int l98_spec_accept_temp_noalloc(const float *p, const float *q, int x, int voca
  * matrix-core kernel; returns 0 (1 on a bad argument or a device error). */
 int l98_gemm_q8(const int8_t *w, const float *ws, int N, int K, const int8_t *xq, const float *xqs, int M,
                 float *out);
+/* ---- paged key-value cache (no reference counterpart) ----
+ * A cache of attention rows in pages that sequences share, and causal
+ * grouped-query attention over it, on arrays that the caller holds in device
+ * memory; beside the sessions' own caches (lz_state_alloc), which are
+ * contiguous and belong to one session.  Results are not the sessions' serial
+ * sums: they are held to the formula within the rounding of the types.
+ *
+ * Every function with an errbuf returns 0, or -LZErr with a message
+ * (-LZ_ERR_NULL_ARG: an argument, -LZ_ERR_FORWARD: a device error).  The work
+ * is enqueued on `stream` (a hipStream_t; NULL: the null stream), which belongs
+ * to the current device, as do all arrays; nothing is allocated, no call
+ * waits, and all of them may be captured into a HIP graph (host arrays are
+ * read before the call returns).  Calls keep nothing between them, so they
+ * may overlap where their arrays do not. */
+#define L98_KV_Q8 LZ_KVF_Q8   /* int8 codes, one float scale per 32 numbers: the sessions' format */
+#define L98_KV_BF16 1
+#define L98_F32 0             /* types of the rows and outputs */
+#define L98_BF16 1
+/* A pool: n_pages pages of page_rows (a power of two, 16 to 1024) rows for
+ * each of n_layers layers, n_kv_heads (<= 1024) heads and K and V, of width
+ * head_dim (32, 64 or 128).  data: l98_kv_page_bytes(pool) * n_pages bytes,
+ * 16-byte aligned; page after page, in a page layer after layer, in a layer's
+ * block K [head][row][dim], V [head][row][dim], and for Q8 the float scales
+ * of K [head][dim / 32][row] and of V.  A Q8 number x of a group of 32 is held
+ * as the byte 128 + rint(x * (127 / max|x|)), its group's scale is
+ * max|x| * (1 / 127) (1 where that is below 1e-30 or max|x| is NaN, with all
+ * bytes 128).  Q8 rows order their bytes as the attention reads them:
+ * dimension 32 c + 8 h + j of K at byte h (dim / 4) + 8 c + j (j < 8, h < 4),
+ * dimension 16 t + n of V at byte n (dim / 16) + t (n < 16). */
+typedef struct {
+    void *data;
+    int format;                    /* L98_KV_Q8 or L98_KV_BF16 */
+    int n_layers, n_pages, page_rows, n_kv_heads, head_dim;
+} L98KvPool;
+/* The sequences of one call, in device arrays that the kernels read when they
+ * run: table[i * table_stride + k] (k < table_pages) is the page of sequence
+ * i's rows k * page_rows .. (an entry outside [0, n_pages) has no rows: they
+ * are not written, read as zeros and attended by nobody); kv_len[i] its
+ * length, the call's new rows included; row0[i] .. row0[i + 1] - 1 the places
+ * of its new rows in the call's arrays, the last of them at position
+ * kv_len[i] - 1.  n_rows: the rows of those arrays; a place outside them is
+ * left alone, and so are places that no sequence has.  max_rows and max_len:
+ * bounds of a sequence's new rows and of kv_len, which size the launch; rows
+ * and positions past them are left out.  n_seq <= 65535. */
+typedef struct {
+    const int *table;
+    long long table_stride;
+    int table_pages;
+    const int *kv_len, *row0;
+    int n_seq, n_rows, max_rows, max_len;
+} L98KvBatch;
+/* Rows [place][head][dim] in device memory, strides in elements, dim's 1. */
+typedef struct {
+    void *p;
+    long long row_stride, head_stride;
+} L98KvRows;
+
+/* Bytes of a page over all layers (a pool's page_bytes * n_pages is its
+ * size), or -LZErr for a pool outside the limits; data may be NULL here. */
+long long l98_kv_page_bytes(const L98KvPool *pool);
+/* The batch's new rows of K and V (n_kv_heads heads each) into the pages of
+ * `layer`; pages written by one call must be different ones (a page that two
+ * sequences share is copied before one of them writes: l98_kv_pages_extend). */
+int l98_kv_append(const L98KvPool *pool, int layer, const L98KvBatch *b, const L98KvRows *k, const L98KvRows *v,
+                  int dtype, void *stream, char *errbuf, int errlen);
+/* The new rows' places of k and v get what the pages hold for them (zeros
+ * where there is no page); a batch whose row0 spans whole sequences reads
+ * them whole. */
+int l98_kv_read(const L98KvPool *pool, int layer, const L98KvBatch *b, const L98KvRows *k, const L98KvRows *v,
+                int dtype, void *stream, char *errbuf, int errlen);
+/* out[place][h] = sum_j p_j v_j / sum_j p_j over the positions j up to the
+ * new row's own that exist, p_j = exp(scale * (q[place][h] . k_j)), K and V of
+ * head h / (n_heads / n_kv_heads); a row with no such position gets zeros.
+ * Softmax and sums in fp32.  A row never depends on positions behind its own,
+ * whatever bits they hold; one that attends a row with infinities or NaN gets
+ * such values.  n_heads: a multiple of n_kv_heads, at most 16 times it.  out
+ * may be q.  ws: l98_kv_attend_ws_bytes bytes of device memory (NULL where
+ * that is 0), 16-byte aligned, of any content, for this call alone until it
+ * has run: calls or graphs that share it run one after the other. */
+long long l98_kv_attend_ws_bytes(const L98KvPool *pool, const L98KvBatch *b, int n_heads, int dtype);
+int l98_kv_attend(const L98KvPool *pool, int layer, const L98KvBatch *b, const L98KvRows *q, const L98KvRows *out,
+                  int n_heads, int dtype, float scale, void *ws, long long ws_bytes, void *stream, char *errbuf,
+                  int errlen);
+/* Page dst[i] gets page src[i]'s bytes (all layers), i < n; host arrays.  The
+ * pages of dst are different, and none of them is in src. */
+int l98_kv_copy_pages(const L98KvPool *pool, const int *src, const int *dst, int n, void *stream, char *errbuf,
+                      int errlen);
+
+/* The pages' book-keeping, on the host: sequences as lists of pages with
+ * counted references, the lowest free page taken first.  One thread at a time
+ * per handle.  Sequence ids are small integers, reused after a free; -LZErr
+ * on a bad argument (6) or where the pages do not suffice (7; nothing has
+ * changed then). */
+typedef struct L98KvPages L98KvPages;
+L98KvPages *l98_kv_pages_open(int n_pages, int page_rows);   /* NULL on a bad argument */
+void l98_kv_pages_close(L98KvPages *h);
+/* A sequence of no rows; its id. */
+int l98_kv_pages_new(L98KvPages *h);
+/* A sequence that shares the first n_rows rows of seq; its id. */
+int l98_kv_pages_fork(L98KvPages *h, int seq, int n_rows);
+/* Makes seq n rows longer.  Where its last page has room but is shared, the
+ * rows go to a copy: returns 1 with the page to copy in *src and its place in
+ * *dst (l98_kv_copy_pages, before anything is appended), else 0. */
+int l98_kv_pages_extend(L98KvPages *h, int seq, int n, int *src, int *dst);
+/* Drops seq's rows from n_rows on (a rejected draft), or all of it. */
+int l98_kv_pages_trim(L98KvPages *h, int seq, int n_rows);
+int l98_kv_pages_free(L98KvPages *h, int seq);
+int l98_kv_pages_len(const L98KvPages *h, int seq);
+/* seq's pages, up to cap of them, into out; their count. */
+int l98_kv_pages_table(const L98KvPages *h, int seq, int *out, int cap);
+int l98_kv_pages_unused(const L98KvPages *h);
+/* Moves the pages in use to the lowest numbers: the copies to make in
+ * src / dst (cap entries, at most min(pages in use, unused)), their count;
+ * every sequence's pages are the new ones at once. */
+int l98_kv_pages_compact(L98KvPages *h, int *src, int *dst, int cap);
 /* Device and build facts, for logs. */
 const char *l98_device_name(void);
 /* Seconds of device time of the last l98_generate call's round loop

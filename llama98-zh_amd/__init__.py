@@ -77,6 +77,21 @@ class L98SynthConfig(C.Structure):
         ("mtp_n_draft", C.c_int)]
 
 
+class L98KvPool(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("format", C.c_int), ("n_layers", C.c_int), ("n_pages", C.c_int),
+                ("page_rows", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int)]
+
+
+class L98KvBatch(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("table_stride", C.c_longlong), ("table_pages", C.c_int),
+                ("kv_len", C.c_void_p), ("row0", C.c_void_p), ("n_seq", C.c_int), ("n_rows", C.c_int),
+                ("max_rows", C.c_int), ("max_len", C.c_int)]
+
+
+class L98KvRows(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("row_stride", C.c_longlong), ("head_stride", C.c_longlong)]
+
+
 _P = C.c_void_p
 _IP = C.POINTER(C.c_int)
 _FP = C.POINTER(C.c_float)
@@ -151,6 +166,27 @@ HIP_API = [
     ("l98_gemv_argmax", C.c_int, [C.c_void_p, _FP, C.c_int, C.c_int, C.c_int, C.c_void_p, _FP, C.c_int, C.c_int,
                                   _FP, _IP]),
     ("l98_gemm_q8", C.c_int, [C.c_void_p, _FP, C.c_int, C.c_int, C.c_void_p, _FP, C.c_int, _FP]),
+    ("l98_kv_page_bytes", C.c_longlong, [C.POINTER(L98KvPool)]),
+    ("l98_kv_append", C.c_int, [C.POINTER(L98KvPool), C.c_int, C.POINTER(L98KvBatch), C.POINTER(L98KvRows),
+                                C.POINTER(L98KvRows), C.c_int, _P, C.c_char_p, C.c_int]),
+    ("l98_kv_read", C.c_int, [C.POINTER(L98KvPool), C.c_int, C.POINTER(L98KvBatch), C.POINTER(L98KvRows),
+                              C.POINTER(L98KvRows), C.c_int, _P, C.c_char_p, C.c_int]),
+    ("l98_kv_attend_ws_bytes", C.c_longlong, [C.POINTER(L98KvPool), C.POINTER(L98KvBatch), C.c_int, C.c_int]),
+    ("l98_kv_attend", C.c_int, [C.POINTER(L98KvPool), C.c_int, C.POINTER(L98KvBatch), C.POINTER(L98KvRows),
+                                C.POINTER(L98KvRows), C.c_int, C.c_int, C.c_float, _P, C.c_longlong, _P, C.c_char_p,
+                                C.c_int]),
+    ("l98_kv_copy_pages", C.c_int, [C.POINTER(L98KvPool), _IP, _IP, C.c_int, _P, C.c_char_p, C.c_int]),
+    ("l98_kv_pages_open", _P, [C.c_int, C.c_int]),
+    ("l98_kv_pages_close", None, [_P]),
+    ("l98_kv_pages_new", C.c_int, [_P]),
+    ("l98_kv_pages_fork", C.c_int, [_P, C.c_int, C.c_int]),
+    ("l98_kv_pages_extend", C.c_int, [_P, C.c_int, C.c_int, _IP, _IP]),
+    ("l98_kv_pages_trim", C.c_int, [_P, C.c_int, C.c_int]),
+    ("l98_kv_pages_free", C.c_int, [_P, C.c_int]),
+    ("l98_kv_pages_len", C.c_int, [_P, C.c_int]),
+    ("l98_kv_pages_table", C.c_int, [_P, C.c_int, _IP, C.c_int]),
+    ("l98_kv_pages_unused", C.c_int, [_P]),
+    ("l98_kv_pages_compact", C.c_int, [_P, _IP, _IP, C.c_int]),
     ("l98_device_name", C.c_char_p, []),
     ("l98_last_loop_seconds", C.c_double, []),
 ]
@@ -573,3 +609,210 @@ class Engine:
             raise RuntimeError(f"l98_generate failed: {n}")
         self.last_rng = samp.rng_state if samp is not None else None   # sampler state after the run
         return toks[:min(n, cap)], ke[:nr.value], na[:nr.value]
+
+
+# ------------------------------------------------ paged key-value cache ---
+
+KV_FORMATS = {"q8": 0, "bf16": 1}
+_KV_TYPES = {"torch.float32": 0, "torch.bfloat16": 1}
+
+
+def _kv_stream(stream, like):
+    """A hipStream_t: the caller's (an integer, or an object with cuda_stream),
+    or the current stream of the tensor's device."""
+    if stream is None:
+        import torch
+        return torch.cuda.current_stream(like.device).cuda_stream
+    return getattr(stream, "cuda_stream", stream)
+
+
+def _kv_type(t, name):
+    code = _KV_TYPES.get(str(t.dtype))
+    if code is None:
+        raise ValueError(f"{name} is {t.dtype}: float32 and bfloat16 are taken")
+    return code
+
+
+def _kv_rows(t, name, n_rows, heads, dim):
+    """L98KvRows of a [rows, heads, dim] tensor on the GPU."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} is not on a GPU")
+    if t.dim() != 3 or t.shape[0] < n_rows or (heads and t.shape[1] != heads) or t.shape[2] != dim:
+        raise ValueError(f"{name} has the shape {tuple(t.shape)}: "
+                         f"[{n_rows} or more, {heads or 'heads'}, {dim}] is taken")
+    if t.stride(2) != 1:
+        raise ValueError(f"{name}'s last dimension has the stride {t.stride(2)}: 1 is taken")
+    return L98KvRows(t.data_ptr(), t.stride(0), t.stride(1))
+
+
+class KvBatch:
+    """The sequences of a call (L98KvBatch): int32 tensors on the GPU, table
+    [sequences, pages], kv_len [sequences], row0 [sequences + 1].  The kernels
+    read them when they run, so their values may change between calls; the
+    bounds n_rows, max_rows and max_len may not."""
+
+    def __init__(self, table, kv_len, row0, n_rows, max_rows, max_len):
+        n_seq = table.shape[0] if table.dim() == 2 else -1
+        for name, t, shape in (("table", table, tuple(table.shape)), ("kv_len", kv_len, (n_seq,)),
+                               ("row0", row0, (n_seq + 1,))):
+            if str(t.dtype) != "torch.int32" or not t.is_cuda or tuple(t.shape) != shape or n_seq < 0:
+                raise ValueError(f"{name} is {t.dtype} {tuple(t.shape)} on {t.device}: "
+                                 f"int32 on a GPU, table [sequences, pages], kv_len [sequences], "
+                                 f"row0 [sequences + 1] are taken")
+            if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
+                raise ValueError(f"{name}'s last dimension has the stride {t.stride(-1)}: 1 is taken")
+        self.table, self.kv_len, self.row0 = table, kv_len, row0
+        self.n_seq, self.n_rows = n_seq, int(n_rows)
+        self.c = L98KvBatch(table.data_ptr(), table.stride(0), table.shape[1], kv_len.data_ptr(), row0.data_ptr(),
+                            n_seq, self.n_rows, int(max_rows), int(max_len))
+
+
+class KvPool:
+    """A paged key-value cache over a tensor of the caller's on the GPU
+    (L98KvPool): append, read, attend and copy_pages are the l98_kv_* calls on
+    the given stream (default: torch's current one).  They raise ValueError
+    for arguments and RuntimeError for device errors."""
+
+    def __init__(self, data, fmt, page_rows, n_kv_heads, head_dim, n_layers=1):
+        if fmt not in KV_FORMATS:
+            raise ValueError(f"format {fmt!r}: {sorted(KV_FORMATS)} are taken")
+        self.lib = hip_lib()
+        self.c = L98KvPool(None, KV_FORMATS[fmt], n_layers, 1, page_rows, n_kv_heads, head_dim)
+        self.page_bytes = self.lib.l98_kv_page_bytes(C.byref(self.c))
+        if self.page_bytes < 0:
+            raise ValueError(f"a pool of {n_layers} layers, pages of {page_rows} rows, {n_kv_heads} heads of "
+                             f"{head_dim} is outside the limits")
+        if not data.is_cuda or not data.is_contiguous():
+            raise ValueError("the pool's tensor is not contiguous on a GPU")
+        n_pages = data.numel() * data.element_size() // self.page_bytes
+        if not 1 <= n_pages < 2 ** 31:
+            raise ValueError(f"the pool's tensor holds {n_pages} pages of {self.page_bytes} bytes")
+        self.data, self.n_pages = data, n_pages
+        self.c.data, self.c.n_pages = data.data_ptr(), n_pages
+        self.n_kv_heads, self.head_dim = n_kv_heads, head_dim
+
+    @staticmethod
+    def page_bytes_of(fmt, page_rows, n_kv_heads, head_dim, n_layers=1):
+        """Bytes of a page, for sizing the tensor."""
+        c = L98KvPool(None, KV_FORMATS[fmt], n_layers, 1, page_rows, n_kv_heads, head_dim)
+        n = hip_lib().l98_kv_page_bytes(C.byref(c))
+        if n < 0:
+            raise ValueError("a pool outside the limits")
+        return n
+
+    @staticmethod
+    def _done(rc, err):
+        if rc:
+            raise (ValueError if rc == -LZ_ERR["NULL_ARG"] else RuntimeError)(err.value.decode(errors="replace"))
+
+    def _pair(self, fn, batch, k, v, layer, stream):
+        code = _kv_type(k, "k")
+        if v.dtype != k.dtype:
+            raise ValueError(f"k is {k.dtype}, v is {v.dtype}")
+        rk = _kv_rows(k, "k", batch.n_rows, self.n_kv_heads, self.head_dim)
+        rv = _kv_rows(v, "v", batch.n_rows, self.n_kv_heads, self.head_dim)
+        err = C.create_string_buffer(256)
+        self._done(fn(self.c, layer, batch.c, rk, rv, code, _kv_stream(stream, k), err, 256), err)
+
+    def append(self, batch, k, v, layer=0, stream=None):
+        """l98_kv_append: the batch's new rows, k and v [rows, n_kv_heads, head_dim]."""
+        self._pair(self.lib.l98_kv_append, batch, k, v, layer, stream)
+
+    def read(self, batch, k, v, layer=0, stream=None):
+        """l98_kv_read: what the pages hold for the batch's new rows, into k and v."""
+        self._pair(self.lib.l98_kv_read, batch, k, v, layer, stream)
+
+    def attend_ws_bytes(self, batch, q):
+        """Bytes of workspace that attend needs for q's heads and type (0: none)."""
+        n = self.lib.l98_kv_attend_ws_bytes(self.c, batch.c, q.shape[1], _kv_type(q, "q"))
+        if n < 0:
+            raise ValueError(f"{q.shape[1]} query heads over {self.n_kv_heads}")
+        return n
+
+    def attend(self, batch, q, out, scale, ws=None, layer=0, stream=None):
+        """l98_kv_attend: q and out [rows, heads, head_dim]; ws a tensor of
+        attend_ws_bytes bytes or more.  Returns out."""
+        code = _kv_type(q, "q")
+        if out.dtype != q.dtype:
+            raise ValueError(f"q is {q.dtype}, out is {out.dtype}")
+        rq = _kv_rows(q, "q", batch.n_rows, 0, self.head_dim)
+        ro = _kv_rows(out, "out", batch.n_rows, q.shape[1], self.head_dim)
+        err = C.create_string_buffer(256)
+        self._done(self.lib.l98_kv_attend(
+            self.c, layer, batch.c, rq, ro, q.shape[1], code, scale, ws.data_ptr() if ws is not None else None,
+            ws.numel() * ws.element_size() if ws is not None else 0, _kv_stream(stream, q), err, 256), err)
+        return out
+
+    def copy_pages(self, src, dst, stream=None):
+        """l98_kv_copy_pages: host lists of page numbers."""
+        src, dst = np.ascontiguousarray(src, np.int32), np.ascontiguousarray(dst, np.int32)
+        if src.ndim != 1 or src.shape != dst.shape:
+            raise ValueError("src and dst are lists of one length")
+        err = C.create_string_buffer(256)
+        self._done(self.lib.l98_kv_copy_pages(self.c, _ip(src), _ip(dst), len(src), _kv_stream(stream, self.data),
+                                              err, 256), err)
+
+
+class KvPages:
+    """The pages' book-keeping (L98KvPages): which sequence has which pages."""
+
+    def __init__(self, n_pages, page_rows):
+        self.lib = hip_lib()
+        self.h = self.lib.l98_kv_pages_open(n_pages, page_rows)
+        if not self.h:
+            raise ValueError(f"{n_pages} pages of {page_rows} rows")
+        self.n_pages = n_pages
+
+    def close(self):
+        if self.h:
+            self.lib.l98_kv_pages_close(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _ok(self, rc):
+        if rc == -LZ_ERR["STATE_ALLOC"]:
+            raise MemoryError("not enough pages")
+        if rc < 0:
+            raise ValueError("no such sequence or length")
+        return rc
+
+    def new(self):
+        return self._ok(self.lib.l98_kv_pages_new(self.h))
+
+    def fork(self, seq, n_rows):
+        return self._ok(self.lib.l98_kv_pages_fork(self.h, seq, n_rows))
+
+    def extend(self, seq, n):
+        """Returns the page copies to make first: ([src], [dst]), empty or one."""
+        a, b = C.c_int(), C.c_int()
+        n = self._ok(self.lib.l98_kv_pages_extend(self.h, seq, n, C.byref(a), C.byref(b)))
+        return ([a.value], [b.value]) if n else ([], [])
+
+    def trim(self, seq, n_rows):
+        self._ok(self.lib.l98_kv_pages_trim(self.h, seq, n_rows))
+
+    def free(self, seq):
+        self._ok(self.lib.l98_kv_pages_free(self.h, seq))
+
+    def len(self, seq):
+        return self._ok(self.lib.l98_kv_pages_len(self.h, seq))
+
+    def table(self, seq):
+        n = self._ok(self.lib.l98_kv_pages_table(self.h, seq, None, 0))
+        out = np.zeros(n, np.int32)
+        self._ok(self.lib.l98_kv_pages_table(self.h, seq, _ip(out), n))
+        return out
+
+    def unused(self):
+        return self._ok(self.lib.l98_kv_pages_unused(self.h))
+
+    def compact(self):
+        """Returns the page copies to make: (src, dst)."""
+        src, dst = np.zeros(self.n_pages, np.int32), np.zeros(self.n_pages, np.int32)
+        n = self._ok(self.lib.l98_kv_pages_compact(self.h, _ip(src), _ip(dst), self.n_pages))
+        return src[:n], dst[:n]
