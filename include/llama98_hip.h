@@ -438,7 +438,7 @@ int l98_gemm_q8(const int8_t *w, const float *ws, int N, int K, const int8_t *xq
  * waits, and all of them may be captured into a HIP graph (host arrays are
  * read before the call returns).  Calls keep nothing between them, so they
  * may overlap where their arrays do not. */
-#define L98_KV_Q8 LZ_KVF_Q8   /* int8 codes, one float scale per 32 numbers: the sessions' format */
+#define L98_KV_Q8 LZ_KVF_Q8   /* int8 codes, one float scale per 32 numbers, as the sessions' */
 #define L98_KV_BF16 1
 #define L98_F32 0             /* types of the rows and outputs */
 #define L98_BF16 1
@@ -448,8 +448,8 @@ int l98_gemm_q8(const int8_t *w, const float *ws, int N, int K, const int8_t *xq
  * 16-byte aligned; page after page, in a page layer after layer, in a layer's
  * block K [head][row][dim], V [head][row][dim], and for Q8 the float scales
  * of K [head][dim / 32][row] and of V.  A Q8 number x of a group of 32 is held
- * as the byte 128 + rint(x * (127 / max|x|)), its group's scale is
- * max|x| * (1 / 127) (1 where that is below 1e-30 or max|x| is NaN, with all
+ * as the byte 128 + rint(x * (127 * (1 / max|x|))), every step in fp32, its
+ * group's scale is max|x| * (1 / 127) (1 where that is below 1e-30 or max|x| is NaN, with all
  * bytes 128).  Q8 rows order their bytes as the attention reads them:
  * dimension 32 c + 8 h + j of K at byte h (dim / 4) + 8 c + j (j < 8, h < 4),
  * dimension 16 t + n of V at byte n (dim / 16) + t (n < 16). */

@@ -1,10 +1,10 @@
 // Rows into and out of the paged key-value cache, and copies of its pages.
 //
-// A Q8 row is the engine's: groups of 32, scale max|x| / 127, codes rounded
-// half to even (q8_scale_inv and d_q8_round, so a row appended here holds the
-// bits that the engine's own cache holds for it), stored as code + 128 in the
-// order that the matrix instructions of the attention read (include/
-// llama98_hip.h).  All three kernels only move bytes: their bound is HBM.
+// A Q8 row is the engine's kind: groups of 32, scale max|x| / 127, codes
+// rounded half to even (d_q8_round), stored as code + 128 in the order that
+// the matrix instructions of the attention read (include/llama98_hip.h).  All three kernels only move bytes: their bound is HBM.
+#include <limits.h>
+
 #include "l98_devmath.h"
 #include "l98_kv.h"
 
@@ -88,6 +88,16 @@ __device__ __forceinline__ long long kv_scale_at(const KvPages &p, const KvUnit 
            ((((((long long)u.which * p.hk + u.head) * (D / 32)) + g) << p.shift) + u.off) * 4;
 }
 
+// q8_scale_inv with the factor 127 * (1 / max) instead of 127 / max: what a
+// torch program that fills pages itself gets from 127.0 / max.  (Some of the
+// factors differ in the last bit, and with them about one code in a million
+// by one.)
+__device__ __forceinline__ void kv_scale_inv(float amax, float *sg, float *inv) {
+    float unused;
+    q8_scale_inv(amax, sg, &unused);
+    *inv = unused == 0.0f ? 0.0f : 127.0f * (1.0f / amax);
+}
+
 __device__ __forceinline__ uint32_t max_over(uint32_t v, int lanes) {    // over aligned groups of `lanes`
     for (int o = 1; o < lanes; o <<= 1) {
         const uint32_t y = __shfl_xor(v, o);
@@ -142,7 +152,7 @@ __global__ __launch_bounds__(KV_THREADS) void k_kv_append(KvPages p, KvSeqs b, K
     }
 #pragma unroll
     for (int g = 0; g < E / 2; g++) {
-        q8_scale_inv(f_from_u(am[g]), &sg, &inv);
+        kv_scale_inv(f_from_u(am[g]), &sg, &inv);
         if (live && (u.which == 0 ? g == 0 && u.lane % (32 / E) == 0 : u.lane == 0))
             *(float *)(u.page + kv_scale_at<D>(p, u, u.which == 0 ? u.lane * E / 32 : g)) = sg;
 #pragma unroll
@@ -232,7 +242,9 @@ static int kv_vec(const KvRows &r, int es, int unit) {
     } while (0)
 #define KV_ROWS_DISPATCH(K)                                                                                \
     const long long units = (long long)b.max_rows * p.hk * 2;                                              \
-    const dim3 grid((unsigned)((units + KV_THREADS / 16 - 1) / (KV_THREADS / 16)), b.n_seq);               \
+    const long long blocks = (units + KV_THREADS / 16 - 1) / (KV_THREADS / 16);                            \
+    if (blocks > INT_MAX) return -1;                                                                       \
+    const dim3 grid((unsigned)blocks, b.n_seq);                                                            \
     if (p.d == 32) KV_ROWS_D(K, 32);                                                                       \
     else if (p.d == 64) KV_ROWS_D(K, 64);                                                                  \
     else if (p.d == 128) KV_ROWS_D(K, 128);                                                                \

@@ -62,7 +62,7 @@ def quant(x):
     s = (am * np.float32(1.0 / 127.0)).astype(np.float32)
     live = (am > 0) & ~(s < np.float32(1e-30))
     with np.errstate(divide="ignore", over="ignore", invalid="ignore"):
-        inv = np.where(live, np.float32(127.0) / am, np.float32(0)).astype(np.float32)
+        inv = np.where(live, np.float32(127.0) * (np.float32(1.0) / am), np.float32(0)).astype(np.float32)
     code = np.clip(np.rint(g * inv[..., None]), -127, 127)
     return code, np.where(live, s, np.float32(1)).astype(np.float32)
 
