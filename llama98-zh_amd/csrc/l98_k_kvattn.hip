@@ -30,42 +30,12 @@
 
 #include "l98_devmath.h"
 #include "l98_kv.h"
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+#include "l98_kvattn.h"
 
 #define FEW_THREADS 256
 #define FEW_WAVES (FEW_THREADS / 64)
 #define FEW_KEYS 32               // of one wave at a time
 
-__device__ __forceinline__ float kv_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ float ninf() { return -__builtin_inff(); }
-
-// bytes `b0` of lo and `b1` of hi, each minus 128, times 2^-9, as two fp16
-__device__ __forceinline__ uint32_t codes2(uint32_t hi, uint32_t lo, uint32_t sel) {
-    const uint32_t u = __builtin_amdgcn_perm(hi, lo, sel);
-    f16x2 x;
-    __builtin_memcpy(&x, &u, 4);
-    const f16x2 a = {(_Float16)32768.0f, (_Float16)32768.0f}, c = {(_Float16)-0.25f, (_Float16)-0.25f};
-    x = __builtin_elementwise_fma(x, a, c);
-    uint32_t r;
-    __builtin_memcpy(&r, &x, 4);
-    return r;
-}
-template <class V> __device__ __forceinline__ V as(u32x4 x) {
-    V v;
-    __builtin_memcpy(&v, &x, 16);
-    return v;
-}
-template <class E> __device__ __forceinline__ uint32_t pack2(E a, E b) {
-    E x[2] = {a, b};
-    uint32_t r;
-    __builtin_memcpy(&r, x, 4);
-    return r;
-}
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
@@ -394,13 +364,6 @@ __device__ __forceinline__ void few_tile(FewAcc<D, Q8, BF, MT> &A, FewTile<D, Q8
     }
 }
 
-// Partial results in the workspace: of (row, head, split) D floats, then the
-// pairs (M, sum).
-struct KvParts {
-    float *o, *ml;
-    int splits;
-};
-
 template <int D, bool Q8, bool BF, int MT>
 __global__ __launch_bounds__(FEW_THREADS, D == 128 && MT == 2 ? 1 : 2) void k_kv_few(KvPages p, KvSeqs b, KvRows q, KvRows out, int heads, int group,
                                                            float scale2, int chunk, int tiles, KvParts w) {
@@ -593,17 +556,28 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_kv_join(KvSeqs b, KvRows out, 
 
 namespace {
 
-struct Plan {
-    int mt, tiles, chunk, splits;
-};
-Plan plan_few(const KvPages &p, const KvSeqs &b, int heads) {
-    Plan x;
+// How a call's work is cut.  rows: of a block's tile; tiles: of a sequence and
+// kv head; chunk: keys of a block; splits: blocks of a tile.
+KvPlan plan(const KvPages &p, const KvSeqs &b, int heads, int bf16) {
+    KvPlan x;
     const long long rows = (long long)b.max_rows * (heads / p.hk);
-    x.mt = rows <= 16 ? 1 : 2;
-    x.tiles = (int)((rows + 16 * x.mt - 1) / (16 * x.mt));
+    x.many = bf16 && rows > 128;
+    int unit, least;
+    long long want;
+    if (x.many) {
+        x.rows = (long long)b.n_seq * p.hk * ((rows + 255) / 256) >= 256 ? 256 : 128;
+        unit = 64;
+        least = 512;
+        want = 256;
+    } else {
+        x.rows = rows <= 16 ? 16 : 32;
+        unit = FEW_WAVES * FEW_KEYS;
+        least = 256;
+        want = 768;
+    }
+    x.tiles = (int)((rows + x.rows - 1) / x.rows);
     const long long base = (long long)b.n_seq * p.hk * x.tiles;
-    const int least = 256, unit = FEW_WAVES * FEW_KEYS;
-    long long splits = (768 + base - 1) / base;
+    long long splits = (want + base - 1) / base;
     const long long most = (b.max_len + least - 1) / least;
     splits = splits < most ? splits : most;
     splits = splits > 1 ? splits : 1;
@@ -615,9 +589,22 @@ Plan plan_few(const KvPages &p, const KvSeqs &b, int heads) {
 }
 
 template <int D, bool Q8, bool BF>
-int launch(const KvPages &p, const KvSeqs &b, const KvRows &q, const KvRows &o, int heads, float scale, void *ws,
-           hipStream_t st) {
-    const Plan x = plan_few(p, b, heads);
+int few(const KvPages &p, const KvSeqs &b, const KvRows &q, const KvRows &o, int heads, float scale2, const KvPlan &x,
+        const KvParts &w, hipStream_t st) {
+    const dim3 grid((unsigned)((long long)x.splits * p.hk * x.tiles), b.n_seq);
+    if (x.rows == 16)
+        hipLaunchKernelGGL((k_kv_few<D, Q8, BF, 1>), grid, dim3(FEW_THREADS), 0, st, p, b, q, o, heads, heads / p.hk,
+                           scale2, x.chunk, x.tiles, w);
+    else
+        hipLaunchKernelGGL((k_kv_few<D, Q8, BF, 2>), grid, dim3(FEW_THREADS), 0, st, p, b, q, o, heads, heads / p.hk,
+                           scale2, x.chunk, x.tiles, w);
+    return (int)hipGetLastError();
+}
+
+template <int D>
+int attend(const KvPages &p, int q8, const KvSeqs &b, const KvRows &q, const KvRows &o, int heads, int bf16, float scale,
+           void *ws, hipStream_t st) {
+    const KvPlan x = plan(p, b, heads, bf16);
     KvParts w;
     w.splits = x.splits;
     w.o = (float *)ws;
@@ -625,41 +612,29 @@ int launch(const KvPages &p, const KvSeqs &b, const KvRows &q, const KvRows &o, 
     const float scale2 = scale * 1.44269504088896341f;
     const long long blocks = (long long)x.splits * p.hk * x.tiles, joins = (long long)b.max_rows * heads;
     if (blocks > INT_MAX || joins > INT_MAX) return -1;
-    const dim3 grid((unsigned)blocks, b.n_seq);
-    if (x.mt == 1)
-        hipLaunchKernelGGL((k_kv_few<D, Q8, BF, 1>), grid, dim3(FEW_THREADS), 0, st, p, b, q, o, heads, heads / p.hk,
-                           scale2, x.chunk, x.tiles, w);
-    else
-        hipLaunchKernelGGL((k_kv_few<D, Q8, BF, 2>), grid, dim3(FEW_THREADS), 0, st, p, b, q, o, heads, heads / p.hk,
-                           scale2, x.chunk, x.tiles, w);
-    const int rc = (int)hipGetLastError();
+    int rc;
+    if (x.many) rc = l98k_kv_many(p, q8, b, q, o, heads, scale2, x, w, st);
+    else if (q8) rc = bf16 ? few<D, true, true>(p, b, q, o, heads, scale2, x, w, st)
+                           : few<D, true, false>(p, b, q, o, heads, scale2, x, w, st);
+    else rc = bf16 ? few<D, false, true>(p, b, q, o, heads, scale2, x, w, st)
+                   : few<D, false, false>(p, b, q, o, heads, scale2, x, w, st);
     if (rc || x.splits == 1) return rc;
-    hipLaunchKernelGGL((k_kv_join<D, BF>), dim3((unsigned)joins, b.n_seq), dim3(JOIN_THREADS), 0, st, b, o,
-                       heads, w);
+    if (bf16) hipLaunchKernelGGL((k_kv_join<D, true>), dim3((unsigned)joins, b.n_seq), dim3(JOIN_THREADS), 0, st, b, o, heads, w);
+    else hipLaunchKernelGGL((k_kv_join<D, false>), dim3((unsigned)joins, b.n_seq), dim3(JOIN_THREADS), 0, st, b, o, heads, w);
     return (int)hipGetLastError();
-}
-
-template <int D>
-int launch_d(const KvPages &p, int q8, const KvSeqs &b, const KvRows &q, const KvRows &o, int heads, int bf16, float scale,
-             void *ws, hipStream_t st) {
-    if (q8)
-        return bf16 ? launch<D, true, true>(p, b, q, o, heads, scale, ws, st)
-                    : launch<D, true, false>(p, b, q, o, heads, scale, ws, st);
-    return bf16 ? launch<D, false, true>(p, b, q, o, heads, scale, ws, st)
-                : launch<D, false, false>(p, b, q, o, heads, scale, ws, st);
 }
 
 }  // namespace
 
-extern "C" long long l98k_kv_attend_ws(const KvPages &p, int, const KvSeqs &b, int heads, int) {
-    const Plan x = plan_few(p, b, heads);
+extern "C" long long l98k_kv_attend_ws(const KvPages &p, int, const KvSeqs &b, int heads, int bf16) {
+    const KvPlan x = plan(p, b, heads, bf16);
     return x.splits == 1 ? 0 : (long long)b.n_rows * heads * x.splits * (p.d + 2) * 4;
 }
 
 extern "C" int l98k_kv_attend(const KvPages &p, int q8, const KvSeqs &b, const KvRows &q, const KvRows &o, int heads,
                               int bf16, float scale, void *ws, hipStream_t st) {
-    if (p.d == 32) return launch_d<32>(p, q8, b, q, o, heads, bf16, scale, ws, st);
-    if (p.d == 64) return launch_d<64>(p, q8, b, q, o, heads, bf16, scale, ws, st);
-    if (p.d == 128) return launch_d<128>(p, q8, b, q, o, heads, bf16, scale, ws, st);
+    if (p.d == 32) return attend<32>(p, q8, b, q, o, heads, bf16, scale, ws, st);
+    if (p.d == 64) return attend<64>(p, q8, b, q, o, heads, bf16, scale, ws, st);
+    if (p.d == 128) return attend<128>(p, q8, b, q, o, heads, bf16, scale, ws, st);
     return -1;
 }

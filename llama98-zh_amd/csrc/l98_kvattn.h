@@ -1,0 +1,52 @@
+// What the two attention kernels over the paged cache share.
+#ifndef L98_KVATTN_H
+#define L98_KVATTN_H
+#include "l98_kv.h"
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float kv_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float ninf() { return -__builtin_inff(); }
+
+// bytes `b0` of lo and `b1` of hi, each minus 128, times 2^-9, as two fp16
+__device__ __forceinline__ uint32_t codes2(uint32_t hi, uint32_t lo, uint32_t sel) {
+    const uint32_t u = __builtin_amdgcn_perm(hi, lo, sel);
+    f16x2 x;
+    __builtin_memcpy(&x, &u, 4);
+    const f16x2 a = {(_Float16)32768.0f, (_Float16)32768.0f}, c = {(_Float16)-0.25f, (_Float16)-0.25f};
+    x = __builtin_elementwise_fma(x, a, c);
+    uint32_t r;
+    __builtin_memcpy(&r, &x, 4);
+    return r;
+}
+template <class V> __device__ __forceinline__ V as(u32x4 x) {
+    V v;
+    __builtin_memcpy(&v, &x, 16);
+    return v;
+}
+template <class E> __device__ __forceinline__ uint32_t pack2(E a, E b) {
+    E x[2] = {a, b};
+    uint32_t r;
+    __builtin_memcpy(&r, x, 4);
+    return r;
+}
+
+// Partial results in the workspace: of (row, head, split) D floats, then the
+// pairs (M, sum): the sums are in units of 2^M.
+struct KvParts {
+    float *o, *ml;
+    int splits;
+};
+
+struct KvPlan {
+    bool many;
+    int rows, tiles, chunk, splits;
+};
+
+extern "C" int l98k_kv_many(const KvPages &p, int q8, const KvSeqs &b, const KvRows &q, const KvRows &o, int heads,
+                            float scale2, const KvPlan &x, const KvParts &w, hipStream_t st);
+#endif
