@@ -211,17 +211,17 @@ __global__ __launch_bounds__(KV_THREADS) void k_kv_read(KvPages p, KvSeqs b, KvR
     }
 }
 
-// Whole pages, 16 bytes a lane and load, KV_COPY_UNROLL loads in flight.
+// Whole pages, 16 bytes a lane and load, KV_COPY_UNROLL loads in flight (the
+// index clamped instead of a branch around each load).
 #define KV_COPY_UNROLL 4
 __global__ __launch_bounds__(KV_THREADS) void k_kv_copy(unsigned char *data, long long page_bytes, KvMoves m) {
-    const uint4 *s = (const uint4 *)(data + m.src[blockIdx.y] * page_bytes);
-    uint4 *d = (uint4 *)(data + m.dst[blockIdx.y] * page_bytes);
-    const long long n = page_bytes / 16;
-    const long long i0 = (long long)blockIdx.x * (KV_THREADS * KV_COPY_UNROLL) + threadIdx.x;
-    uint4 x[KV_COPY_UNROLL];
+    typedef uint32_t v4 __attribute__((ext_vector_type(4)));
+    const v4 *s = (const v4 *)(data + m.src[blockIdx.y] * page_bytes);
+    v4 *d = (v4 *)(data + m.dst[blockIdx.y] * page_bytes);
+    const long long n = page_bytes / 16, i0 = (long long)blockIdx.x * (KV_THREADS * KV_COPY_UNROLL) + threadIdx.x;
+    v4 x[KV_COPY_UNROLL];
 #pragma unroll
-    for (int u = 0; u < KV_COPY_UNROLL; u++)
-        if (i0 + u * KV_THREADS < n) x[u] = s[i0 + u * KV_THREADS];
+    for (int u = 0; u < KV_COPY_UNROLL; u++) x[u] = s[i0 + u * KV_THREADS < n ? i0 + u * KV_THREADS : n - 1];
 #pragma unroll
     for (int u = 0; u < KV_COPY_UNROLL; u++)
         if (i0 + u * KV_THREADS < n) d[i0 + u * KV_THREADS] = x[u];

@@ -19,8 +19,7 @@
 // scaled there.  q is scaled by a power of two per row to below 2^15; a bf16
 // row is then exact in fp16, an fp32 row goes as two fp16 parts (22 bits).
 // The weights w = p * (V's scale of the group) are at most 2^15 (the running
-// maximum M bounds s + log2(scale) - 15 instead of s; the sum runs in the same
-// unit), in one fp16 for bf16 rows (a rounding of 2^-11, against 2^-8 of the
+// maximum is of s + log2(scale); the sum runs in the same unit), in one fp16 for bf16 rows (a rounding of 2^-11, against 2^-8 of the
 // output), two parts for fp32 rows.  bf16 caches: q and p in as many bf16
 // parts as their types need: a bf16 q is exact, fp32 takes three (24 bits); p
 // takes two for bf16 rows, three for fp32.
@@ -43,16 +42,6 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// N parts of E whose sum is x to N times E's bits
-template <class E, int N>
-__device__ __forceinline__ void parts(float x, E *o) {
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        o[i] = (E)x;
-        x -= (float)o[i];
-    }
-}
-
 // The shape of the work for one (width, cache, row type).
 template <int D, bool Q8, bool BF>
 struct Few {
@@ -67,16 +56,6 @@ struct Few {
     using V8 = typename std::conditional<Q8, f16x8, bf16x8>::type;
     // a lane's operand element j of contraction c: this dimension of K and q
     static __device__ __forceinline__ int dim(int c, int h) { return Q8 ? c * 32 + h * 8 : h * (D / 4) + c * 8; }
-};
-
-// What a lane holds of 32 keys: K of key t*16 + (lane & 15), V of the eight
-// keys t*16 + 4*(lane >> 4) + i, and 4 of the tile's Q8 scales.
-template <int D, bool Q8, bool BF>
-struct FewTile {
-    using F = Few<D, Q8, BF>;
-    uint32_t k[2][F::KW], v[8][F::VW];
-    f32x4 sc[(2 * F::NG * FEW_KEYS) / 256 ? (2 * F::NG * FEW_KEYS) / 256 : 1];
-    bool there[2];
 };
 
 template <int B>
@@ -101,46 +80,76 @@ __device__ __forceinline__ void load_bytes(const unsigned char *s, uint32_t *o) 
     }
 }
 
-// The 32 keys from `key` on (a multiple of 32, below the sequence's end): both
-// 16-key halves lie within one page each, whose bytes all exist, so positions
-// past the length are read too (and masked where they are used).
+// What a lane holds of a tile of 32 keys: K of key t*16 + (lane & 15), V of the
+// eight keys t*16 + 4*(lane >> 4) + i, and 4 of the tile's Q8 scales.
 template <int D, bool Q8, bool BF>
-__device__ __forceinline__ void few_load(FewTile<D, Q8, BF> &T, const KvPages &p, const int *table, int pages, int kh,
-                                         int key, int len) {
+struct FewTile {
     using F = Few<D, Q8, BF>;
-    const int lane = threadIdx.x & 63, n = lane & 15, h = lane >> 4, rows = 1 << p.shift;
-    const int vo = p.hk << p.shift;                          // V's rows behind K's
-    const unsigned char *pg[2];
-    int off[2];
+    uint32_t k[2][F::KW], v[8][F::VW];
+    f32x4 sc;
+};
+
+// The pages of a tile's two 16-key halves, which each lie within one: all its
+// bytes exist, so positions past the length are read too, and masked where
+// they are used.
+struct FewPages {
+    int id[2];
+};
+__device__ __forceinline__ FewPages few_pages(const KvPages &p, const int *table, int pages, int key) {
+    FewPages x;
 #pragma unroll
     for (int t = 0; t < 2; t++) {
-        const int k = key + 16 * t, at = k >> p.shift;
-        const int id = at < pages ? table[at] : -1;
-        T.there[t] = (unsigned)id < (unsigned)p.n_pages;
-        pg[t] = kv_page(p, T.there[t] ? id : 0);
-        off[t] = (kh << p.shift) + (k & (rows - 1));
+        const int at = (key + 16 * t) >> p.shift;
+        x.id[t] = at < pages ? table[at] : -1;
     }
-#pragma unroll
-    for (int t = 0; t < 2; t++) {
-        load_bytes<F::KB>(pg[t] + (off[t] + n) * (Q8 ? D : 2 * D) + h * F::KB, T.k[t]);
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            load_bytes<F::VB>(pg[t] + (vo + off[t] + h * 4 + i) * (Q8 ? D : 2 * D) + n * F::VB, T.v[t * 4 + i]);
+    return x;
+}
+
+// The addresses of a kv head's tiles: uniform ones per tile half, and what is
+// the lane's own.
+template <int D, bool Q8, bool BF>
+struct FewAddr {
+    using F = Few<D, Q8, BF>;
+    static constexpr uint32_t ROW = Q8 ? D : 2 * D;
+    uint32_t head, v, scales;              // of the page's block: this head's K, V behind K, the scales
+    uint32_t lane_k, lane_v, lane_s;
+    bool second;                           // the lane's scales belong to the second half
+
+    __device__ __forceinline__ FewAddr(const KvPages &p, int kh) {
+        const uint32_t lane = threadIdx.x & 63, n = lane & 15, h = lane >> 4;
+        head = ((uint32_t)kh << p.shift) * ROW;
+        v = ((uint32_t)p.hk << p.shift) * ROW;
+        scales = 2 * v;
+        lane_k = n * ROW + h * F::KB;
+        lane_v = h * 4 * ROW + n * F::VB;
+        // lane x: 4 keys' scales, x = (which * NG + group) * 8 + key / 4
+        const uint32_t which = (lane / (F::NG * 8)) & 1, g = (lane / 8) % F::NG, k4 = (lane & 7) * 4;
+        second = k4 >= 16;
+        lane_s = ((((which * p.hk + kh) * F::NG + g) << p.shift) + (k4 & 15)) * 4;
     }
-    if (Q8) {
-        // chunk x of the tile's 2 NG 32 / 4 scales: which, group, 4 keys
+    __device__ __forceinline__ const unsigned char *base(const KvPages &p, const FewPages &x, int t) const {
+        return kv_page(p, (unsigned)x.id[t] < (unsigned)p.n_pages ? x.id[t] : 0);
+    }
+    __device__ __forceinline__ uint32_t at(const KvPages &p, int key, int t) const {
+        return (uint32_t)((key + 16 * t) & ((1 << p.shift) - 1));
+    }
+    __device__ __forceinline__ void load_k(FewTile<D, Q8, BF> &T, const KvPages &p, const FewPages &x, int key) const {
 #pragma unroll
-        for (int u = 0; u < (int)(sizeof(T.sc) / 16); u++) {
-            const int x = u * 64 + lane, which = (x / (F::NG * 8)) & 1, g = (x / 8) % F::NG, k4 = (x & 7) * 4, t = k4 >> 4;
-            const unsigned char *s = (t ? pg[1] : pg[0]) + 2 * vo * D +
-                                     (((which * p.hk + kh) * F::NG + g) << p.shift) * 4 +
-                                     (((key + k4) & (rows - 1)) * 4);
-            T.sc[u] = *(const f32x4 *)s;
+        for (int t = 0; t < 2; t++) load_bytes<F::KB>(base(p, x, t) + (head + at(p, key, t) * ROW) + lane_k, T.k[t]);
+    }
+    __device__ __forceinline__ void load_v(FewTile<D, Q8, BF> &T, const KvPages &p, const FewPages &x, int key) const {
 #pragma unroll
-            for (int i = 0; i < 4; i++) T.sc[u][i] = key + k4 + i < len ? T.sc[u][i] : 0.0f;
+        for (int t = 0; t < 2; t++) {
+            const unsigned char *s = base(p, x, t) + (v + head + at(p, key, t) * ROW);
+#pragma unroll
+            for (int i = 0; i < 4; i++) load_bytes<F::VB>(s + i * ROW + lane_v, T.v[t * 4 + i]);
+        }
+        if (Q8) {
+            const unsigned char *s0 = base(p, x, 0) + (scales + at(p, key, 0) * 4), *s1 = base(p, x, 1) + (scales + at(p, key, 1) * 4);
+            T.sc = *(const f32x4 *)((second ? s1 : s0) + lane_s);
         }
     }
-}
+};
 
 __device__ __forceinline__ float max_h(float x) {            // over the four lanes of a query
     x = fmaxf(x, __shfl_xor(x, 16));
@@ -151,6 +160,38 @@ __device__ __forceinline__ float sum_h(float x) {
     return x + __shfl_xor(x, 32);
 }
 
+// the largest of the wave's words, by DPP: over rows of 16, then over the rows
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t x) {
+    auto step = [&](uint32_t y) { x = y > x ? y : x; };
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, true));   // row_shr:1
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, true));
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, true));
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, true));
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, true));   // row_bcast:15 into rows 1, 3
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, true));   // row_bcast:31 into rows 2, 3
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+
+// eight consecutive numbers; without a branch around each load, or they would
+// be waited for one by one
+template <class T>
+__device__ __forceinline__ void load8(const T *s, int vec, float *x) {
+    typedef T vt __attribute__((ext_vector_type(16 / sizeof(T))));
+    constexpr int N = 16 / sizeof(T);
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 8; i += N) {
+            const vt t = *reinterpret_cast<const vt *>(s + i);
+#pragma unroll
+            for (int u = 0; u < N; u++) x[i + u] = (float)t[u];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (float)s[i];
+    }
+}
+
+#define FEW_NONE -3.0e38f         // the running maximum of a row without keys
 template <int D, bool Q8, bool BF, int MT>
 struct FewAcc {
     using F = Few<D, Q8, BF>;
@@ -160,124 +201,119 @@ struct FewAcc {
     int lim[MT];                                             // the row's keys: below this
 };
 
-// One tile of 32 keys.  masked: some row of the block's may not attend some
-// of them, or they are not all there.
+// The scores of a tile, s[m][t][i] of query (lane & 15) and key t*16 + 4*(lane >> 4) + i.
 template <int D, bool Q8, bool BF, int MT>
-__device__ __forceinline__ void few_tile(FewAcc<D, Q8, BF, MT> &A, FewTile<D, Q8, BF> &T, float *sc, int key, int len,
-                                         bool masked) {
+__device__ __forceinline__ void few_scores(const FewAcc<D, Q8, BF, MT> &A, const FewTile<D, Q8, BF> &T, const float *sc,
+                                           f32x4 (&s)[MT][2]) {
     using F = Few<D, Q8, BF>;
-    using E = typename F::E;
     using V8 = typename F::V8;
-    const int lane = threadIdx.x & 63, h = lane >> 4;
-    f32x4 s[MT][2];
-    if (Q8) {
-        // the wave's own part of LDS: written whole, then read by every lane
+    const int h = (threadIdx.x & 63) >> 4;
 #pragma unroll
-        for (int u = 0; u < (int)(sizeof(T.sc) / 16); u++)
-            if (u * 64 + lane < 2 * F::NG * 8) *(f32x4 *)(sc + (u * 64 + lane) * 4) = T.sc[u];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    }
-    float top[MT];
+    for (int m = 0; m < MT; m++)
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
+        for (int t = 0; t < 2; t++) s[m][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int m = 0; m < MT; m++) s[m][t] = f32x4{0, 0, 0, 0};
+    for (int c = 0; c < F::NG; c++) {
+        f32x4 part[MT][2], ks[2];
 #pragma unroll
-        for (int c = 0; c < F::NG; c++) {
+        for (int t = 0; t < 2; t++) {
             u32x4 kx;
             if (Q8) {
+                ks[t] = *(const f32x4 *)(sc + c * FEW_KEYS + t * 16 + h * 4);
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
-                    const uint32_t x = T.k[t][2 * c + w];
-                    kx[2 * w] = codes2(0, x, 0x0c010c00u);
-                    kx[2 * w + 1] = codes2(0, x, 0x0c030c02u);
-                }
-                const f32x4 ks = *(const f32x4 *)(sc + c * FEW_KEYS + t * 16 + h * 4);
-#pragma unroll
-                for (int m = 0; m < MT; m++) {
-                    f32x4 part = {0, 0, 0, 0};
-#pragma unroll
-                    for (int i = 0; i < F::NQ; i++) part = mfma(as<V8>(kx), as<V8>(A.q[m][c][i]), part);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) s[m][t][i] = __builtin_fmaf(part[i], ks[i], s[m][t][i]);
+                    kx[2 * w] = codes2(0, T.k[t][2 * c + w], 0x0c010c00u);
+                    kx[2 * w + 1] = codes2(0, T.k[t][2 * c + w], 0x0c030c02u);
                 }
             } else {
 #pragma unroll
                 for (int w = 0; w < 4; w++) kx[w] = T.k[t][4 * c + w];
+            }
 #pragma unroll
-                for (int m = 0; m < MT; m++)
+            for (int m = 0; m < MT; m++) {
+                if (Q8) part[m][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                    for (int i = 0; i < F::NQ; i++) s[m][t] = mfma(as<V8>(kx), as<V8>(A.q[m][c][i]), s[m][t]);
+                for (int i = 0; i < F::NQ; i++) {
+                    if (Q8) part[m][t] = mfma(as<V8>(kx), as<V8>(A.q[m][c][i]), part[m][t]);
+                    else s[m][t] = mfma(as<V8>(kx), as<V8>(A.q[m][c][i]), s[m][t]);
+                }
             }
         }
+        if (Q8)
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[m][t][i] = __builtin_fmaf(part[m][t][i], ks[t][i], s[m][t][i]);
     }
-    // scores in units of log2, masked; the largest of the row and, for Q8, of V's scales with it
+}
+
+// Softmax of a tile's scores and the products with V.  there: which halves
+// have a page; masked: some row may not attend some of the keys, or they are
+// not all there.
+template <int D, bool Q8, bool BF, int MT>
+__device__ __forceinline__ void few_values(FewAcc<D, Q8, BF, MT> &A, FewTile<D, Q8, BF> &T, const float *sc,
+                                           f32x4 (&s)[MT][2], int key, int len, bool there0, bool there1, bool masked,
+                                           float vex) {
+    using F = Few<D, Q8, BF>;
+    using E = typename F::E;
+    using V8 = typename F::V8;
+    const int h = (threadIdx.x & 63) >> 4;
+    // Q8 weights are p * (V's scale): 2^ex > every scale that the row attends
+    // of the tile (vex: all of them), and s + ex bounds their logarithm.  They
+    // may reach 2^15; a raise of the running maximum brings them to 2^11.
+    // bf16: p up to 2^8, and to 1.
+    constexpr float ROOM = Q8 ? 15.0f : 8.0f, DROP = Q8 ? 11.0f : 0.0f;
+    float cand[MT];
+    bool up = false;
+    if (masked) {
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
-        float mx = ninf();
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                s[m][t][i] *= A.cq[m];
-                if (masked && !(T.there[t] && key + t * 16 + h * 4 + i < A.lim[m])) s[m][t][i] = ninf();
-                mx = fmaxf(mx, s[m][t][i]);
-            }
-        top[m] = mx;
-    }
-    float vmax[8];
-    if (Q8) {
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            f32x4 x = *(const f32x4 *)(sc + F::NG * FEW_KEYS + t * 16 + h * 4);
-#pragma unroll
-            for (int g = 1; g < F::NG; g++) {
-                const f32x4 y = *(const f32x4 *)(sc + (F::NG + g) * FEW_KEYS + t * 16 + h * 4);
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[i] = fmaxf(x[i], y[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) vmax[t * 4 + i] = x[i];
-        }
-    }
-    bool same = true;
-    float keep[MT];
-#pragma unroll
-    for (int m = 0; m < MT; m++) {
-        float mt = max_h(top[m]);
-        if (Q8) {
-            // 2^ex > every V scale that the row attends; M = s + ex - 15
-            float x = 0.0f;
+        for (int m = 0; m < MT; m++) {
+            float vx = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const bool in = !masked || (T.there[i >> 2] && key + (i >> 2) * 16 + h * 4 + (i & 3) < A.lim[m]);
-                x = fmaxf(x, in ? vmax[i] : 0.0f);
+                const int k = (i >> 2) * 16 + h * 4 + (i & 3);
+                const bool in = (i < 4 ? there0 : there1) && key + k < A.lim[m];
+                s[m][i >> 2][i & 3] = in ? s[m][i >> 2][i & 3] : ninf();
+                if (Q8)
+#pragma unroll
+                    for (int g = 0; g < F::NG; g++) vx = fmaxf(vx, in ? sc[(F::NG + g) * FEW_KEYS + k] : 0.0f);
             }
-            x = max_h(x);
-            mt += (float)((int)(u_from_f(x) >> 23) - 126 - 15);
+            cand[m] = Q8 ? (float)((int)(u_from_f(vx) >> 23) - 126) : 0.0f;
         }
-        const float mn = fmaxf(A.m[m], mt), mu = mn == ninf() ? 0.0f : mn;
-        keep[m] = kv_exp2(A.m[m] - mu);
-        same = same && mn == A.m[m];
-        A.m[m] = mn;
-        float l = 0.0f;
+    } else {
 #pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                s[m][t][i] = kv_exp2(s[m][t][i] - mu);
-                l += s[m][t][i];
-            }
-        A.l[m] = __builtin_fmaf(A.l[m], keep[m], l);
+        for (int m = 0; m < MT; m++) cand[m] = vex;
     }
-    if (!__all(same)) {
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+    for (int m = 0; m < MT; m++) {
+        float mx = s[m][0][0];
 #pragma unroll
-            for (int d = 0; d < F::NT; d++) A.o[m][d] *= keep[m];
+        for (int i = 1; i < 8; i++) mx = fmaxf(mx, s[m][i >> 2][i & 3]);
+        cand[m] = __builtin_fmaf(mx, A.cq[m], cand[m]);
+        up = up || cand[m] > A.m[m] + ROOM;
     }
+    if (__any(up)) {
+        // each row by itself: its bits must not depend on the tile's other rows
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            const float c = max_h(cand[m]);
+            const bool mine = c > A.m[m] + ROOM;
+            const float f = mine ? kv_exp2(A.m[m] - (c - DROP)) : 1.0f;
+            A.m[m] = mine ? c - DROP : A.m[m];
+            A.l[m] *= f;
+#pragma unroll
+            for (int d = 0; d < F::NT; d++) A.o[m][d] *= f;
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            s[m][i >> 2][i & 3] = kv_exp2(__builtin_fmaf(s[m][i >> 2][i & 3], A.cq[m], -A.m[m]));
+            A.l[m] += s[m][i >> 2][i & 3];
+        }
     if (!Q8 && masked) {
         // A key that some row may not attend must not reach it as 0 * NaN: its
         // V becomes zero; where it has a value that is not finite, the rows
@@ -288,92 +324,86 @@ __device__ __forceinline__ void few_tile(FewAcc<D, Q8, BF, MT> &A, FewTile<D, Q8
 #pragma unroll
             for (int w = 0; w < F::VW; w++)
                 bad = bad || (T.v[i][w] & 0x7F80u) == 0x7F80u || (T.v[i][w] & 0x7F800000u) == 0x7F800000u;
-            const bool any = ((__ballot(bad) >> (16 * h)) & 0xFFFFull) != 0;
+            const bool any = ((__ballot(bad) >> (16 * h)) & 0xFFFFull) != 0, there = i < 4 ? there0 : there1;
             const int k = key + (i >> 2) * 16 + h * 4 + (i & 3);
-            const bool drop = any || k >= len || !T.there[i >> 2];
+            const bool drop = any || k >= len || !there;
 #pragma unroll
             for (int w = 0; w < F::VW; w++) T.v[i][w] = drop ? 0u : T.v[i][w];
 #pragma unroll
             for (int m = 0; m < MT; m++)
-                if (any && T.there[i >> 2] && k < A.lim[m]) A.l[m] = __builtin_nanf("");
+                if (any && there && k < A.lim[m]) A.l[m] = __builtin_nanf("");
         }
     }
-    if (Q8) {
-#pragma unroll
-        for (int g = 0; g < F::NG; g++) {
-            u32x4 w[MT][F::NP];
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const f32x4 vs = *(const f32x4 *)(sc + (F::NG + g) * FEW_KEYS + t * 16 + h * 4);
-#pragma unroll
-                for (int m = 0; m < MT; m++) {
-                    E e[4][F::NP];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        float x = s[m][t][i] * vs[i];
-                        // a scale that is not finite, of a key that the row may not attend
-                        if (masked && !(T.there[t] && key + t * 16 + h * 4 + i < A.lim[m])) x = 0.0f;
-                        parts<E, F::NP>(x, e[i]);
-                    }
-#pragma unroll
-                    for (int k = 0; k < F::NP; k++) {
-                        w[m][k][2 * t] = pack2(e[0][k], e[1][k]);
-                        w[m][k][2 * t + 1] = pack2(e[2][k], e[3][k]);
-                    }
-                }
-            }
-#pragma unroll
-            for (int d = 2 * g; d < 2 * g + 2; d++) {
-                u32x4 vx;
-                constexpr uint32_t base = 0x0c040c00u;
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    vx[i] = codes2(T.v[2 * i + 1][d / 4], T.v[2 * i][d / 4], base + (uint32_t)(d & 3) * 0x00010001u);
-#pragma unroll
-                for (int m = 0; m < MT; m++)
-#pragma unroll
-                    for (int k = 0; k < F::NP; k++) A.o[m][d] = mfma(as<V8>(vx), as<V8>(w[m][k]), A.o[m][d]);
-            }
-        }
-    } else {
-        u32x4 w[MT][F::NP];
+    u32x4 w[MT][F::NP];
+    auto weights = [&](const f32x4 (&vs)[2]) {
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                E e[4][F::NP];
-#pragma unroll
-                for (int i = 0; i < 4; i++) parts<E, F::NP>(s[m][t][i], e[i]);
-#pragma unroll
-                for (int k = 0; k < F::NP; k++) {
-                    w[m][k][2 * t] = pack2(e[0][k], e[1][k]);
-                    w[m][k][2 * t + 1] = pack2(e[2][k], e[3][k]);
+            for (int i = 0; i < 8; i += 2) {
+                const int t = i >> 2, e = i & 3;
+                float a = s[m][t][e], b = s[m][t][e + 1];
+                if (Q8) {
+                    a *= vs[t][e];
+                    b *= vs[t][e + 1];
+                    if (masked) {                            // 0 * a scale that is not finite
+                        const bool there = t ? there1 : there0;
+                        const int k = key + t * 16 + h * 4 + e;
+                        a = there && k < A.lim[m] ? a : 0.0f;
+                        b = there && k + 1 < A.lim[m] ? b : 0.0f;
+                    }
                 }
+                uint32_t x[F::NP];
+                parts2<E, F::NP>(a, b, x);
+#pragma unroll
+                for (int k = 0; k < F::NP; k++) w[m][k][i / 2] = x[k];
             }
+    };
+    auto product = [&](int d, const u32x4 &vx) {
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int k = 0; k < F::NP; k++) A.o[m][d] = mfma(as<V8>(vx), as<V8>(w[m][k]), A.o[m][d]);
+    };
+    if (Q8) {
+#pragma unroll
+        for (int g = 0; g < F::NG; g++) {
+            f32x4 vs[2];
+#pragma unroll
+            for (int t = 0; t < 2; t++) vs[t] = *(const f32x4 *)(sc + (F::NG + g) * FEW_KEYS + t * 16 + h * 4);
+            weights(vs);
+#pragma unroll
+            for (int d = 2 * g; d < 2 * g + 2; d++) {
+                u32x4 vx;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    vx[i] = codes2(T.v[2 * i + 1][d / 4], T.v[2 * i][d / 4], 0x0c040c00u + (uint32_t)(d & 3) * 0x00010001u);
+                product(d, vx);
+            }
+        }
+    } else {
+        const f32x4 one[2] = {};
+        weights(one);
 #pragma unroll
         for (int d = 0; d < F::NT; d++) {
             u32x4 vx;
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 vx[i] = __builtin_amdgcn_perm(T.v[2 * i + 1][d / 2], T.v[2 * i][d / 2], d & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int k = 0; k < F::NP; k++) A.o[m][d] = mfma(as<V8>(vx), as<V8>(w[m][k]), A.o[m][d]);
+            product(d, vx);
         }
     }
 }
 
 template <int D, bool Q8, bool BF, int MT>
-__global__ __launch_bounds__(FEW_THREADS, D == 128 && MT == 2 ? 1 : 2) void k_kv_few(KvPages p, KvSeqs b, KvRows q, KvRows out, int heads, int group,
-                                                           float scale2, int chunk, int tiles, KvParts w) {
+__global__ __launch_bounds__(FEW_THREADS, 2) void k_kv_few(KvPages p, KvSeqs b, KvRows q, KvRows out, int heads, int group,
+                                                           float scale2, int chunk, int tiles, int vec, KvParts w) {
     using F = Few<D, Q8, BF>;
     using E = typename F::E;
     using T = typename std::conditional<BF, __bf16, float>::type;
     constexpr int ROWS = 16 * MT, SC = 2 * F::NG * FEW_KEYS;
-    __shared__ float so[FEW_WAVES * ROWS * D];               // the loop's scales, then the waves' results
+    __shared__ __align__(16) float so[FEW_WAVES * ROWS * D]; // the loop's scales, then the waves' results
     __shared__ float sm[FEW_WAVES][ROWS], sl[FEW_WAVES][ROWS];
-    static_assert(SC * FEW_WAVES <= FEW_WAVES * ROWS * D, "the scales fit");
+    static_assert(SC <= ROWS * D, "the scales fit");
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, h = lane >> 4;
     // splits of a tile next to each other, the tiles with the most keys first
     const int seq = blockIdx.y, split = blockIdx.x % w.splits, y = blockIdx.x / w.splits;
@@ -390,6 +420,25 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 && MT == 2 ? 1 : 2) void k_kv
     int k1 = k0 + chunk;
     k1 = k1 < end ? k1 : end;
     const int *table = b.table + seq * b.stride;
+    if (k0 >= k1 && w.splits > 1) {                          // no keys: the join skips this part
+        const int row = tile * ROWS + threadIdx.x, j = row / group, r = s.r0 + j;
+        if (threadIdx.x < ROWS && j < nr && (unsigned)r < (unsigned)b.n_rows) {
+            const long long at = ((long long)r * heads + kh * group + row % group) * w.splits + split;
+            *(float2 *)(w.ml + 2 * at) = make_float2(ninf(), 0.0f);
+        }
+        return;
+    }
+
+    const FewAddr<D, Q8, BF> addr(p, kh);
+    FewTile<D, Q8, BF> tl;
+    FewPages pg = {{-1, -1}};
+    const int step = FEW_WAVES * FEW_KEYS;
+    int key = k0 + wave * FEW_KEYS;
+    if (key < k1) {
+        pg = few_pages(p, table, b.pages, key);
+        addr.load_k(tl, p, pg, key);
+        addr.load_v(tl, p, pg, key);
+    }
 
     FewAcc<D, Q8, BF, MT> A;
 #pragma unroll
@@ -398,7 +447,7 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 && MT == 2 ? 1 : 2) void k_kv
         const bool on = j < nr && (unsigned)r < (unsigned)b.n_rows;
         const T *src = (const T *)q.p + (on ? r * q.row + (kh * group + row % group) * q.head : 0);
         A.lim[m] = on ? (s.pos0 + j + 1 < s.len ? s.pos0 + j + 1 : s.len) : 0;
-        A.m[m] = ninf();
+        A.m[m] = FEW_NONE;
         A.l[m] = 0.0f;
 #pragma unroll
         for (int d = 0; d < F::NT; d++) A.o[m][d] = f32x4{0, 0, 0, 0};
@@ -406,54 +455,78 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 && MT == 2 ? 1 : 2) void k_kv
         uint32_t big = 0;
 #pragma unroll
         for (int c = 0; c < F::NG; c++)
+            load8(src + F::dim(c, h), vec, x[c]);
+#pragma unroll
+        for (int c = 0; c < F::NG; c++)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                x[c][i] = on ? (float)src[F::dim(c, h) + i] : 0.0f;
+                x[c][i] = on ? x[c][i] : 0.0f;
                 const uint32_t a = u_from_f(x[c][i]) & 0x7FFFFFFFu;
                 big = a > big ? a : big;
             }
-        A.cq[m] = scale2;
-        int e = 0;
+        // a negative scale turns q around, so that the factor of the scores is
+        // not negative; nor zero, so that -inf stays what it is
+        A.cq[m] = fabsf(scale2);
+        float unit = scale2 < 0.0f ? -1.0f : 1.0f;
         if (Q8) {
             uint32_t y = __shfl_xor(big, 16);
             big = y > big ? y : big;
             y = __shfl_xor(big, 32);
             big = y > big ? y : big;
-            e = (int)(big >> 23) - 127 - 14;                 // the row's largest to [2^14, 2^15)
-            A.cq[m] = __builtin_amdgcn_ldexpf(scale2, e + 9);
+            const int e = (int)(big >> 23) - 127 - 14;       // the row's largest to [2^14, 2^15)
+            A.cq[m] = __builtin_amdgcn_ldexpf(A.cq[m], e + 9);
+#pragma unroll
+            for (int c = 0; c < F::NG; c++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[c][i] = __builtin_amdgcn_ldexpf(x[c][i], -e);
         }
+        A.cq[m] = fmaxf(A.cq[m], 1e-37f);
 #pragma unroll
         for (int c = 0; c < F::NG; c++)
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
-                E lo[F::NQ], hi[F::NQ];
-                parts<E, F::NQ>(Q8 ? __builtin_amdgcn_ldexpf(x[c][i], -e) : x[c][i], lo);
-                parts<E, F::NQ>(Q8 ? __builtin_amdgcn_ldexpf(x[c][i + 1], -e) : x[c][i + 1], hi);
+                uint32_t y[F::NQ];
+                parts2<E, F::NQ>(x[c][i] * unit, x[c][i + 1] * unit, y);
 #pragma unroll
-                for (int k = 0; k < F::NQ; k++) A.q[m][c][k][i / 2] = pack2(lo[k], hi[k]);
+                for (int k = 0; k < F::NQ; k++) A.q[m][c][k][i / 2] = y[k];
             }
     }
     // keys below this are attended by every row of the tile
     int all = s.pos0 + j_first + 1;
     all = all < s.len ? all : s.len;
-    float *sc = so + wave * SC;
-    const int step = FEW_WAVES * FEW_KEYS;
-    int key = k0 + wave * FEW_KEYS;
-    if (key < k1) {
-        FewTile<D, Q8, BF> t0, t1;
-        few_load<D, Q8, BF>(t0, p, table, b.pages, kh, key, s.len);
-        for (;;) {
-            const bool m0 = key + FEW_KEYS > all || !(t0.there[0] && t0.there[1]);
-            const int next = key + step;
-            if (next < k1) few_load<D, Q8, BF>(t1, p, table, b.pages, kh, next, s.len);
-            few_tile<D, Q8, BF, MT>(A, t0, sc, key, s.len, m0);
-            if (next >= k1) break;
-            key = next + step;
-            const bool m1 = next + FEW_KEYS > all || !(t1.there[0] && t1.there[1]);
-            if (key < k1) few_load<D, Q8, BF>(t0, p, table, b.pages, kh, key, s.len);
-            few_tile<D, Q8, BF, MT>(A, t1, sc, next, s.len, m1);
-            if (key >= k1) break;
+    float *sc = so + wave * ROWS * D;
+    while (key < k1) {
+        const int next = key + step;
+        const bool there0 = (unsigned)pg.id[0] < (unsigned)p.n_pages, there1 = (unsigned)pg.id[1] < (unsigned)p.n_pages;
+        const bool masked = key + FEW_KEYS > all || !there0 || !there1;
+        float vex = 0.0f;
+        if (Q8) {
+            // the wave's own part of LDS: written whole, then read by every lane
+            if (masked) {
+                const int k4 = key + (lane & 7) * 4;
+#pragma unroll
+                for (int i = 0; i < 4; i++) tl.sc[i] = k4 + i < s.len ? tl.sc[i] : 0.0f;
+            }
+            if (lane < 2 * F::NG * 8) *(f32x4 *)(sc + lane * 4) = tl.sc;
+            if (!masked) {
+                const float x = fmaxf(fmaxf(tl.sc[0], tl.sc[1]), fmaxf(tl.sc[2], tl.sc[3]));
+                vex = (float)((int)(wave_max_bits(lane >= F::NG * 8 && lane < 2 * F::NG * 8 ? u_from_f(x) : 0u) >> 23) - 126);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
+        // the last turn loads its own tile again, without a branch: registers
+        // that are loaded on one of two paths came out of the compiler
+        // overwritten before their last use
+        const int ahead = next < k1 ? next : key;
+        pg = few_pages(p, table, b.pages, ahead);
+        f32x4 x[MT][2];
+        few_scores<D, Q8, BF, MT>(A, tl, sc, x);
+        addr.load_k(tl, p, pg, ahead);
+        few_values<D, Q8, BF, MT>(A, tl, sc, x, key, s.len, there0, there1, masked, vex);
+        addr.load_v(tl, p, pg, ahead);
+        key = next;
     }
     // the four waves' results: scaled to the block's maximum, summed in wave order
 #pragma unroll
@@ -467,10 +540,10 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 && MT == 2 ? 1 : 2) void k_kv
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < MT; m++) {
-        float mx = ninf();
+        float mx = FEW_NONE;
 #pragma unroll
         for (int x = 0; x < FEW_WAVES; x++) mx = fmaxf(mx, sm[x][m * 16 + n]);
-        const float f = kv_exp2(A.m[m] - (mx == ninf() ? 0.0f : mx));
+        const float f = kv_exp2(A.m[m] - mx);
         float *o = so + (wave * ROWS + m * 16 + n) * D;
 #pragma unroll
         for (int d = 0; d < F::NT; d++)
@@ -482,11 +555,11 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 && MT == 2 ? 1 : 2) void k_kv
     const int m = threadIdx.x / PER, d0 = threadIdx.x % PER * DT;
     const int row = tile * ROWS + m, j = row / group, r = s.r0 + j, head = kh * group + row % group;
     if (j >= nr || (unsigned)r >= (unsigned)b.n_rows) return;
-    float mx = ninf(), l = 0.0f, x[DT];
+    float mx = FEW_NONE, l = 0.0f, x[DT];
 #pragma unroll
     for (int y = 0; y < FEW_WAVES; y++) mx = fmaxf(mx, sm[y][m]);
 #pragma unroll
-    for (int y = 0; y < FEW_WAVES; y++) l += sl[y][m] * kv_exp2(sm[y][m] - (mx == ninf() ? 0.0f : mx));
+    for (int y = 0; y < FEW_WAVES; y++) l += sl[y][m] * kv_exp2(sm[y][m] - mx);
 #pragma unroll
     for (int i = 0; i < DT; i++) {
         x[i] = 0.0f;
@@ -496,16 +569,17 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 && MT == 2 ? 1 : 2) void k_kv
     }
     if (w.splits == 1) {
         T *dst = (T *)out.p + r * out.row + head * out.head + d0;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-        for (int i = 0; i < DT; i++) dst[i] = (T)(l == 0.0f ? 0.0f : x[i] / l);
+        for (int i = 0; i < DT; i++) dst[i] = (T)(x[i] * inv);
         return;
     }
     const long long at = ((long long)r * heads + head) * w.splits + split;
     if (d0 == 0) {
-        w.ml[2 * at] = mx;
+        w.ml[2 * at] = mx == FEW_NONE ? ninf() : mx;
         w.ml[2 * at + 1] = l;
     }
-    if (mx != ninf())
+    if (mx != FEW_NONE)
 #pragma unroll
         for (int i = 0; i < DT; i++) w.o[at * D + d0 + i] = x[i];
 }
@@ -513,41 +587,64 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 && MT == 2 ? 1 : 2) void k_kv
 // out = sum over splits of 2^(M_s - M) o_s / sum of 2^(M_s - M) l_s, in split
 // order within a lane and then over the lanes: one block per (row, head).
 #define JOIN_THREADS 256
+#define JOIN_MOST 1024            // splits
 template <int D, bool BF>
 __global__ __launch_bounds__(JOIN_THREADS) void k_kv_join(KvSeqs b, KvRows out, int heads, KvParts w) {
     using T = typename std::conditional<BF, __bf16, float>::type;
-    constexpr int L = D / 4, G = JOIN_THREADS / L;           // lanes of a split, splits at a time
-    __shared__ float so[G][D], sl[G], sm[JOIN_THREADS / 64];
+    constexpr int L = D / 4, G = JOIN_THREADS / L, U = 4;    // lanes of a split, splits at a time, loads in flight
+    __shared__ __align__(16) float so[G][D];
+    __shared__ float sf[JOIN_MOST], sl[JOIN_THREADS / 64], sm[JOIN_THREADS / 64];
     const int j = blockIdx.x / heads, head = blockIdx.x % heads, seq = blockIdx.y, tid = threadIdx.x;
     const int r0 = b.row0[seq], nr = b.row0[seq + 1] - r0, r = r0 + j;
     if (j >= nr || (unsigned)r >= (unsigned)b.n_rows) return;
     const long long at = ((long long)r * heads + head) * w.splits;
-    float mx = ninf();
-    for (int i = tid; i < w.splits; i += JOIN_THREADS) mx = fmaxf(mx, w.ml[2 * (at + i)]);
+    float m[JOIN_MOST / JOIN_THREADS], l[JOIN_MOST / JOIN_THREADS], mx = ninf(), sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < JOIN_MOST / JOIN_THREADS; u++) {
+        const int i = tid + u * JOIN_THREADS;
+        const float2 x = i < w.splits ? *(const float2 *)(w.ml + 2 * (at + i)) : make_float2(ninf(), 0.0f);
+        m[u] = x.x;
+        l[u] = x.y;
+        mx = fmaxf(mx, x.x);
+    }
     for (int x = 1; x < 64; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
     if ((tid & 63) == 0) sm[tid >> 6] = mx;
     __syncthreads();
     for (int i = 0; i < JOIN_THREADS / 64; i++) mx = fmaxf(mx, sm[i]);
+#pragma unroll
+    for (int u = 0; u < JOIN_MOST / JOIN_THREADS; u++) {
+        const int i = tid + u * JOIN_THREADS;
+        const float f = m[u] == ninf() ? 0.0f : kv_exp2(m[u] - mx);
+        if (i < w.splits) sf[i] = m[u] == ninf() ? -1.0f : f;      // -1: no keys, its o is not written
+        sum += m[u] == ninf() ? 0.0f : l[u] * f;
+    }
+    for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+    if ((tid & 63) == 0) sl[tid >> 6] = sum;
+    __syncthreads();
     const int g = tid / L, d = tid % L * 4;
     f32x4 acc = {0, 0, 0, 0};
-    float l = 0.0f;
-    for (int i = g; i < w.splits; i += G) {
-        const float mi = w.ml[2 * (at + i)];
-        if (mi == ninf()) continue;                          // no keys: its o is not written
-        const float f = kv_exp2(mi - mx);
-        l += w.ml[2 * (at + i) + 1] * f;
-        acc += *(const f32x4 *)(w.o + (at + i) * D + d) * f;
+    for (int i0 = g; i0 < w.splits; i0 += U * G) {
+        f32x4 x[U];
+        float f[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = i0 + u * G < w.splits ? i0 + u * G : i0;
+            f[u] = i0 + u * G < w.splits ? sf[i] : -1.0f;
+            x[u] = *(const f32x4 *)(w.o + (at + i) * D + d);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[e] += f[u] == -1.0f ? 0.0f : x[u][e] * f[u];
     }
     *(f32x4 *)&so[g][d] = acc;
-    if (d == 0) sl[g] = l;
     __syncthreads();
     if (tid < D) {
         float x = 0.0f, y = 0.0f;
 #pragma unroll
-        for (int i = 0; i < G; i++) {
-            x += so[i][tid];
-            y += sl[i];
-        }
+        for (int i = 0; i < G; i++) x += so[i][tid];
+#pragma unroll
+        for (int i = 0; i < JOIN_THREADS / 64; i++) y += sl[i];
         ((T *)out.p + r * out.row + head * out.head)[tid] = (T)(y == 0.0f ? 0.0f : x / y);
     }
 }
@@ -580,6 +677,7 @@ KvPlan plan(const KvPages &p, const KvSeqs &b, int heads, int bf16) {
     long long splits = (want + base - 1) / base;
     const long long most = (b.max_len + least - 1) / least;
     splits = splits < most ? splits : most;
+    splits = splits < JOIN_MOST ? splits : JOIN_MOST;
     splits = splits > 1 ? splits : 1;
     const long long chunk = ((b.max_len + splits - 1) / splits + unit - 1) / unit * unit;
     x.chunk = (int)(chunk > unit ? chunk : unit);
@@ -591,13 +689,14 @@ KvPlan plan(const KvPages &p, const KvSeqs &b, int heads, int bf16) {
 template <int D, bool Q8, bool BF>
 int few(const KvPages &p, const KvSeqs &b, const KvRows &q, const KvRows &o, int heads, float scale2, const KvPlan &x,
         const KvParts &w, hipStream_t st) {
+    const int es = BF ? 2 : 4, vec = (uintptr_t)q.p % 16 == 0 && q.row * es % 16 == 0 && q.head * es % 16 == 0;
     const dim3 grid((unsigned)((long long)x.splits * p.hk * x.tiles), b.n_seq);
     if (x.rows == 16)
         hipLaunchKernelGGL((k_kv_few<D, Q8, BF, 1>), grid, dim3(FEW_THREADS), 0, st, p, b, q, o, heads, heads / p.hk,
-                           scale2, x.chunk, x.tiles, w);
+                           scale2, x.chunk, x.tiles, vec, w);
     else
         hipLaunchKernelGGL((k_kv_few<D, Q8, BF, 2>), grid, dim3(FEW_THREADS), 0, st, p, b, q, o, heads, heads / p.hk,
-                           scale2, x.chunk, x.tiles, w);
+                           scale2, x.chunk, x.tiles, vec, w);
     return (int)hipGetLastError();
 }
 

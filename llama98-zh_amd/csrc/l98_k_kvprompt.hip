@@ -179,8 +179,8 @@ __device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, ManyLds<D> &L, i
         if (Q8) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const _Float16 f = (_Float16)__builtin_amdgcn_ldexpf(S.ks[u][i], 15 - ek);
-                const uint32_t ff = pack2(f, f);
+                const float f = __builtin_amdgcn_ldexpf(S.ks[u][i], 15 - ek);
+                const uint32_t ff = pack2<_Float16>(f, f);
                 u32x4 o;
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
@@ -227,8 +227,8 @@ __device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, ManyLds<D> &L, i
             for (int g = 0; g < T::SG; g++)
 #pragma unroll
                 for (int w = 0; w < 2; w++)
-                    f[g][w] = pack2((_Float16)__builtin_amdgcn_ldexpf(S.vs[u][g][2 * w], 15 - ev),
-                                    (_Float16)__builtin_amdgcn_ldexpf(S.vs[u][g][2 * w + 1], 15 - ev));
+                    f[g][w] = pack2<_Float16>(__builtin_amdgcn_ldexpf(S.vs[u][g][2 * w], 15 - ev),
+                                              __builtin_amdgcn_ldexpf(S.vs[u][g][2 * w + 1], 15 - ev));
         }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -354,7 +354,8 @@ __global__ __launch_bounds__(NW * 64, 2) void k_kv_many(KvPages p, KvSeqs b, KvR
                 ev = evn;
             }
             ek = ekn;
-            if (next < k1) many_load<D, Q8, NT>(S, p, table, b.pages, kh, next, s.len);
+            // (the last turn loads its own tile again, without a branch)
+            many_load<D, Q8, NT>(S, p, table, b.pages, kh, next < k1 ? next : key, s.len);
             if (key < wend) {
                 f32x16 st[2] = {};
 #pragma unroll
@@ -405,13 +406,13 @@ __global__ __launch_bounds__(NW * 64, 2) void k_kv_many(KvPages p, KvSeqs b, KvR
                 for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
-                        V8 pw;
+                        u32x4 pw;
 #pragma unroll
-                        for (int i = 0; i < 8; i++) pw[i] = (E)st[t][u * 8 + i];
+                        for (int i = 0; i < 4; i++) pw[i] = pack2<E>(st[t][u * 8 + 2 * i], st[t][u * 8 + 2 * i + 1]);
 #pragma unroll
                         for (int d = 0; d < DT; d++) {
                             const u32x4 a = *(const u32x4 *)&L.v[buf][chunk_at<8>(d * 32 + n, (t * 2 + u) * 2 + h) * 8];
-                            o[d] = mfma32(as<V8>(a), pw, o[d]);
+                            o[d] = mfma32(as<V8>(a), as<V8>(pw), o[d]);
                         }
                     }
             }
@@ -442,8 +443,8 @@ __global__ __launch_bounds__(NW * 64, 2) void k_kv_many(KvPages p, KvSeqs b, KvR
             for (int i = 0; i < 16; i += 4) {
                 const int d0 = d * 32 + (i >> 2) * 8 + h * 4;
                 uint2 t;
-                t.x = pack2((__bf16)(o[d][i] * inv), (__bf16)(o[d][i + 1] * inv));
-                t.y = pack2((__bf16)(o[d][i + 2] * inv), (__bf16)(o[d][i + 3] * inv));
+                t.x = pack2<__bf16>(o[d][i] * inv, o[d][i + 1] * inv);
+                t.y = pack2<__bf16>(o[d][i + 2] * inv, o[d][i + 3] * inv);
                 if (vec) {
                     *(uint2 *)(dst + d0) = t;
                 } else {

@@ -28,11 +28,31 @@ template <class V> __device__ __forceinline__ V as(u32x4 x) {
     __builtin_memcpy(&v, &x, 16);
     return v;
 }
-template <class E> __device__ __forceinline__ uint32_t pack2(E a, E b) {
-    E x[2] = {a, b};
+template <class E> struct Pair;
+template <> struct Pair<_Float16> { typedef f16x2 type; };
+template <> struct Pair<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(2))); };
+// two floats rounded to E, half to even, as one instruction
+template <class E> __device__ __forceinline__ typename Pair<E>::type round2(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_convertvector((f32x2){a, b}, typename Pair<E>::type);
+}
+template <class E> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const typename Pair<E>::type x = round2<E>(a, b);
     uint32_t r;
-    __builtin_memcpy(&r, x, 4);
+    __builtin_memcpy(&r, &x, 4);
     return r;
+}
+// N words whose halves' sums are a and b to N times E's bits
+template <class E, int N> __device__ __forceinline__ void parts2(float a, float b, uint32_t *o) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const typename Pair<E>::type x = round2<E>(a, b);
+        __builtin_memcpy(&o[i], &x, 4);
+        if (i + 1 < N) {
+            a -= (float)x[0];
+            b -= (float)x[1];
+        }
+    }
 }
 
 // Partial results in the workspace: of (row, head, split) D floats, then the
