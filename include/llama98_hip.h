@@ -444,7 +444,7 @@ int l98_gemm_q8(const int8_t *w, const float *ws, int N, int K, const int8_t *xq
 #define L98_BF16 1
 /* A pool: n_pages pages of page_rows (a power of two, 16 to 1024) rows for
  * each of n_layers layers, n_kv_heads (<= 1024) heads and K and V, of width
- * head_dim (32, 64 or 128).  data: l98_kv_page_bytes(pool) * n_pages bytes,
+ * head_dim (32, 64 or 128), a page of less than 64 GiB.  data: l98_kv_page_bytes(pool) * n_pages bytes,
  * 16-byte aligned; page after page, in a page layer after layer, in a layer's
  * block K [head][row][dim], V [head][row][dim], and for Q8 the float scales
  * of K [head][dim / 32][row] and of V.  A Q8 number x of a group of 32 is held

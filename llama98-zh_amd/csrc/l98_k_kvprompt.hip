@@ -15,7 +15,7 @@
 // of the largest so far (V; the sums are rescaled when it grows), two roundings
 // of 2^-11 against the output's 2^-8; numbers below 2^-27 of the largest lose
 // bits.  bf16 caches are used as they are.  Weights are rounded to the same 16
-// bits, their sum is taken of the unrounded ones in fp32.
+// bits, and their sum, in fp32, is of the rounded ones.
 //
 // The running maximum is raised only where a tile exceeds it by 2^8 (weights
 // stay below 2^8): the sums are rescaled a few times per row instead of once
@@ -50,12 +50,38 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {   // packed f
 __device__ __forceinline__ float finite_or_0(float x) {
     return (u_from_f(x) & 0x7F800000u) == 0x7F800000u ? 0.0f : x;
 }
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
-    return x;
+__device__ __forceinline__ int exp_above(uint32_t bits) { return (int)(bits >> 23) - 126; }   // 2^this > the float >= 0
+// the wave's largest of each half of x, in both halves of the result: by DPP, over rows of 16, then over the rows
+__device__ __forceinline__ uint32_t wave_max2(uint32_t x) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    auto step = [&](uint32_t y) {
+        u16x2 p, q;
+        __builtin_memcpy(&p, &x, 4);
+        __builtin_memcpy(&q, &y, 4);
+        p = __builtin_elementwise_max(p, q);
+        __builtin_memcpy(&x, &p, 4);
+    };
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, true));   // row_shr:1
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, true));
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, true));
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, true));
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, true));   // row_bcast:15 into rows 1, 3
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, true));   // row_bcast:31 into rows 2, 3
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
-__device__ __forceinline__ int exp_above(float x) { return (int)(u_from_f(x) >> 23) - 126; }   // 2^this > x >= 0
+// c + the two fp16 or bf16 numbers of x
+template <class E> __device__ __forceinline__ float add2(uint32_t x, float c);
+template <> __device__ __forceinline__ float add2<_Float16>(uint32_t x, float c) {
+    f16x2 v;
+    __builtin_memcpy(&v, &x, 4);
+    return __builtin_amdgcn_fdot2(v, (f16x2){(_Float16)1.0f, (_Float16)1.0f}, c, false);
+}
+template <> __device__ __forceinline__ float add2<__bf16>(uint32_t x, float c) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    bf16x2 v;
+    __builtin_memcpy(&v, &x, 4);
+    return __builtin_amdgcn_fdot2_f32_bf16(v, (bf16x2){(__bf16)1.0f, (__bf16)1.0f}, c, false);
+}
 
 // A 64-key tile's share of a thread, on its way from the pages to LDS.
 template <int D, bool Q8, int NT>
@@ -71,86 +97,100 @@ struct Stage {
     uint32_t v[VU][4][ES];
     float ks[Q8 ? KU : 1][2];
     f32x4 vs[Q8 ? VU : 1][SG];
-    float kmax, vmax;                                        // of this lane's share of the tile's scales
+    f32x4 kall, vall;                                        // this lane's share of all the tile's scales
     uint32_t hole;                                           // bit i: keys 16 i .. of the tile have no page
 };
 
-template <int D, bool Q8, int NT>
-__device__ __forceinline__ void many_load(Stage<D, Q8, NT> &S, const KvPages &p, const int *table, int pages, int kh,
-                                          int key, int len) {
-    using T = Stage<D, Q8, NT>;
-    const int rows = 1 << p.shift, vo = p.hk << p.shift, tid = threadIdx.x;
-    const unsigned char *pg[4];
-    S.hole = 0;
+// The pages of a tile's four 16-key quarters (uniform: scalar loads).
+struct ManyPages {
+    int id[4];
+    uint32_t hole;
+};
+__device__ __forceinline__ ManyPages many_pages(const KvPages &p, const int *table, int pages, int key) {
+    ManyPages x;
+    x.hole = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {                            // uniform: scalar loads
+    for (int i = 0; i < 4; i++) {
         const int at = (key + 16 * i) >> p.shift, id = at < pages ? table[at] : -1;
         const bool there = (unsigned)id < (unsigned)p.n_pages;
-        if (!there) S.hole |= 1u << i;
-        pg[i] = kv_page(p, there ? id : 0);
+        if (!there) x.hole |= 1u << i;
+        x.id[i] = there ? id : 0;
     }
-    auto page = [&](int k) {                                 // of the tile's key k
-        const unsigned char *a = k & 16 ? pg[1] : pg[0], *c = k & 16 ? pg[3] : pg[2];
-        return k & 32 ? c : a;
+    return x;
+}
+
+template <int D, bool Q8, int NT>
+__device__ __forceinline__ void many_load(Stage<D, Q8, NT> &S, const KvPages &p, const ManyPages &pg, int kh, int key) {
+    using T = Stage<D, Q8, NT>;
+    const uint32_t rows = 1u << p.shift, vo = (uint32_t)p.hk << p.shift, tid = threadIdx.x, at0 = (uint32_t)key & (rows - 1);
+    const uint32_t unit = (uint32_t)(p.page_bytes >> 4), scales = 2 * vo * D, head = (uint32_t)kh << p.shift;
+    S.hole = pg.hole;
+    const uint32_t id0 = pg.id[0], id1 = pg.id[1], id2 = pg.id[2], id3 = pg.id[3];
+    auto page = [=](uint32_t k) {                            // of the tile's key k
+        const uint32_t a = k & 16 ? id1 : id0, c = k & 16 ? id3 : id2, id = k & 32 ? c : a;
+        return p.data + (((uint64_t)id * unit) << 4);
     };
-    const int at0 = key & (rows - 1);
-    auto row = [&](int k) { return (kh << p.shift) + ((at0 + k) & (rows - 1)); };
+    auto row = [&](uint32_t k) { return (at0 + k) & (rows - 1); };
 #pragma unroll
     for (int u = 0; u < T::KU; u++) {
-        const int x = u * NT + tid;
-        if (T::KT % NT && x >= T::KT) break;
-        const int k = x / T::KROW, c = x % T::KROW;
+        const uint32_t x = u * NT + tid, k = x / T::KROW % MANY_KEYS, c = x % T::KROW;
         const unsigned char *pk = page(k);
-        S.k[u] = *(const u32x4 *)(pk + row(k) * (D * T::ES) + c * 16);
+        S.k[u] = *(const u32x4 *)(pk + ((head + row(k)) * (D * T::ES) + c * 16));
         if (Q8) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int g = (2 * c + i) % T::G;            // chunk h G + g holds 8 numbers of group g
-                S.ks[u][i] = *(const float *)(pk + 2 * vo * D + ((((kh * T::G) + g) << p.shift) + ((at0 + k) & (rows - 1))) * 4);
+                const uint32_t g = (2 * c + i) % T::G;       // chunk h G + g holds 8 numbers of group g
+                S.ks[u][i] = *(const float *)(pk + (scales + (((kh * T::G + g) << p.shift) + row(k)) * 4));
             }
         }
     }
 #pragma unroll
     for (int u = 0; u < T::VU; u++) {
-        const int x = u * NT + tid;
-        if (T::VT % NT && x >= T::VT) break;
-        const int k = x / T::VROW * 4, c = x % T::VROW;
-        const unsigned char *pv = page(k);
+        const uint32_t x = u * NT + tid, k = x / T::VROW * 4 % MANY_KEYS, c = x % T::VROW;
+        const unsigned char *pv = page(k), *s = pv + ((vo + head + row(k)) * (D * T::ES) + c * 4 * T::ES);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const unsigned char *s = pv + (vo + row(k) + i) * (D * T::ES) + c * 4 * T::ES;
             if (Q8) {
-                S.v[u][i][0] = *(const uint32_t *)s;
+                S.v[u][i][0] = *(const uint32_t *)(s + i * (D * T::ES));
             } else {
-                const uint2 y = *(const uint2 *)s;
+                const uint2 y = *(const uint2 *)(s + i * (D * T::ES));
                 S.v[u][i][0] = y.x;
                 S.v[u][i][T::ES - 1] = y.y;
             }
         }
         if (Q8) {
+            const uint32_t g = D == 32 ? 0 : (4 * c) % (D / 16) / 2;         // byte n (D/16) + t: group t / 2
 #pragma unroll
-            for (int i = 0; i < T::SG; i++) {
-                const int g = D == 32 ? 0 : (4 * c) % (D / 16) / 2 + i;      // byte n (D/16) + t: group t / 2
-                S.vs[u][i] = *(const f32x4 *)(pv + 2 * vo * D +
-                                              (((((p.hk + kh) * T::G) + g) << p.shift) + ((at0 + k) & (rows - 1))) * 4);
-            }
+            for (int i = 0; i < T::SG; i++)
+                S.vs[u][i] = *(const f32x4 *)(pv + (scales + ((((p.hk + kh) * T::G + g + i) << p.shift) + row(k)) * 4));
         }
     }
     if (Q8) {
         // every wave over all of the tile's scales, so that all know the same exponents
-        const int lane = tid & 63, k = (lane & 15) * 4, g = (lane >> 4) % T::G;
-        const unsigned char *pp = page(k);
-        const int at = (at0 + k) & (rows - 1);
-        const f32x4 a = *(const f32x4 *)(pp + 2 * vo * D + (((kh * T::G + g) << p.shift) + at) * 4);
-        const f32x4 c = *(const f32x4 *)(pp + 2 * vo * D + ((((p.hk + kh) * T::G + g) << p.shift) + at) * 4);
-        S.kmax = S.vmax = 0.0f;
+        const uint32_t lane = tid & 63, k = (lane & 15) * 4, g = (lane >> 4) % T::G;
+        const unsigned char *s = page(k) + (scales + (((kh * T::G + g) << p.shift) + row(k)) * 4);
+        S.kall = *(const f32x4 *)s;
+        S.vall = *(const f32x4 *)(s + (vo * T::G) * 4);
+    }
+}
+
+// Exponents above the tile's K and V scales, of the keys that exist.
+template <int D, bool Q8, int NT>
+__device__ __forceinline__ void many_exps(Stage<D, Q8, NT> &S, int key, int len, bool masked, int &ek, int &ev) {
+    if (masked) {
+        const int k = (threadIdx.x & 15) * 4;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const bool in = key + k + i < len && !(S.hole >> (k >> 4) & 1);
-            S.kmax = fmaxf(S.kmax, in ? finite_or_0(a[i]) : 0.0f);
-            S.vmax = fmaxf(S.vmax, in ? finite_or_0(c[i]) : 0.0f);
+            S.kall[i] = in ? finite_or_0(S.kall[i]) : 0.0f;
+            S.vall[i] = in ? finite_or_0(S.vall[i]) : 0.0f;
         }
     }
+    const float a = fmaxf(fmaxf(S.kall[0], S.kall[1]), fmaxf(S.kall[2], S.kall[3]));
+    const float c = fmaxf(fmaxf(S.vall[0], S.vall[1]), fmaxf(S.vall[2], S.vall[3]));
+    const uint32_t x = wave_max2(__builtin_amdgcn_perm(u_from_f(a), u_from_f(c), 0x07060302u));
+    ek = exp_above(x & 0xFFFF0000u);
+    ev = exp_above(x << 16);
 }
 
 // 16-byte chunk c of row r (of CH chunks) in LDS: rows of less than 256 bytes
@@ -174,8 +214,8 @@ __device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, ManyLds<D> &L, i
 #pragma unroll
     for (int u = 0; u < T::KU; u++) {
         const int x = u * NT + tid;
-        if (T::KT % NT && x >= T::KT) break;
         const int k = x / T::KROW, c = x % T::KROW;
+        if (T::KT % NT && x >= T::KT) break;
         if (Q8) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -327,19 +367,20 @@ __global__ __launch_bounds__(NW * 64, 2) void k_kv_many(KvPages p, KvSeqs b, KvR
         if (threadIdx.x < 6) L.bad[threadIdx.x >> 1][threadIdx.x & 1] = 0;
         __syncthreads();
         int evn = ev, ekn = 0;
-        auto bounds = [&](Stage<D, Q8, NT> &S) {
+        auto bounds = [&](Stage<D, Q8, NT> &S, int key, bool masked) {
             if (!Q8) return;
-            ekn = exp_above(wave_max(S.kmax));
-            const int x = exp_above(wave_max(S.vmax));
+            int x;
+            many_exps<D, Q8, NT>(S, key, s.len, masked, ekn, x);
             evn = evn > x ? evn : x;
         };
         Stage<D, Q8, NT> S;
-        bool masked = k0 + MANY_KEYS > all, next_masked;
-        many_load<D, Q8, NT>(S, p, table, b.pages, kh, k0, s.len);
-        bounds(S);
-        masked = masked || S.hole;
+        ManyPages pg = many_pages(p, table, b.pages, k0);
+        bool masked = k0 + MANY_KEYS > all || pg.hole, next_masked;
+        many_load<D, Q8, NT>(S, p, pg, kh, k0);
         uint32_t hole = S.hole;
+        bounds(S, k0, masked);
         many_store<D, Q8, NT>(S, L, 0, 0, k0, s.len, masked, ekn, evn);
+        pg = many_pages(p, table, b.pages, k0 + MANY_KEYS < k1 ? k0 + MANY_KEYS : k0);
         __syncthreads();
         for (int key = k0, buf = 0, turn = 0; key < k1; key += MANY_KEYS, buf ^= 1) {
             const int next = key + MANY_KEYS, turn1 = turn == 2 ? 0 : turn + 1;
@@ -355,7 +396,8 @@ __global__ __launch_bounds__(NW * 64, 2) void k_kv_many(KvPages p, KvSeqs b, KvR
             }
             ek = ekn;
             // (the last turn loads its own tile again, without a branch)
-            many_load<D, Q8, NT>(S, p, table, b.pages, kh, next < k1 ? next : key, s.len);
+            many_load<D, Q8, NT>(S, p, pg, kh, next < k1 ? next : key);
+            pg = many_pages(p, table, b.pages, next + MANY_KEYS < k1 ? next + MANY_KEYS : key);
             if (key < wend) {
                 f32x16 st[2] = {};
 #pragma unroll
@@ -400,7 +442,6 @@ __global__ __launch_bounds__(NW * 64, 2) void k_kv_many(KvPages p, KvSeqs b, KvR
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
                         st[t][i] = kv_exp2(__builtin_fmaf(st[t][i], c, -mu));
-                        l += st[t][i];
                     }
 #pragma unroll
                 for (int t = 0; t < 2; t++)
@@ -408,7 +449,10 @@ __global__ __launch_bounds__(NW * 64, 2) void k_kv_many(KvPages p, KvSeqs b, KvR
                     for (int u = 0; u < 2; u++) {
                         u32x4 pw;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) pw[i] = pack2<E>(st[t][u * 8 + 2 * i], st[t][u * 8 + 2 * i + 1]);
+                        for (int i = 0; i < 4; i++) {
+                            pw[i] = pack2<E>(st[t][u * 8 + 2 * i], st[t][u * 8 + 2 * i + 1]);
+                            l = add2<E>(pw[i], l);
+                        }
 #pragma unroll
                         for (int d = 0; d < DT; d++) {
                             const u32x4 a = *(const u32x4 *)&L.v[buf][chunk_at<8>(d * 32 + n, (t * 2 + u) * 2 + h) * 8];
@@ -417,9 +461,9 @@ __global__ __launch_bounds__(NW * 64, 2) void k_kv_many(KvPages p, KvSeqs b, KvR
                     }
             }
             if (next < k1) {
-                bounds(S);
                 hole = S.hole;
                 next_masked = next + MANY_KEYS > all || hole;
+                bounds(S, next, next_masked);
                 many_store<D, Q8, NT>(S, L, buf ^ 1, turn1, next, s.len, next_masked, ekn, evn);
                 masked = next_masked;
             }

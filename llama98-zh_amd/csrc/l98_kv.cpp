@@ -26,12 +26,15 @@ int fail(char *errbuf, int errlen, int code, const char *fmt, ...) {
 }
 #define BAD(...) return fail(errbuf, errlen, LZ_ERR_NULL_ARG, __VA_ARGS__)
 
-bool pool_ok(const L98KvPool *p) {
+bool pool_in_limits(const L98KvPool *p) {
     return p && (p->format == L98_KV_Q8 || p->format == L98_KV_BF16) && p->n_layers >= 1 && p->n_layers <= 1024 &&
            p->n_pages >= 1 && p->page_rows >= 16 && p->page_rows <= 1024 && !(p->page_rows & (p->page_rows - 1)) &&
            p->n_kv_heads >= 1 && p->n_kv_heads <= 1024 &&
            (p->head_dim == 32 || p->head_dim == 64 || p->head_dim == 128);
 }
+long long layer_bytes(const L98KvPool *p);
+// the kernels count a page in 16-byte units of 32 bits
+bool pool_ok(const L98KvPool *p) { return pool_in_limits(p) && layer_bytes(p) * p->n_layers < (1LL << 36); }
 long long layer_bytes(const L98KvPool *p) {
     const long long n = (long long)p->n_kv_heads * p->page_rows * p->head_dim;
     return p->format == L98_KV_Q8 ? 2 * (n + n / 32 * 4) : 4 * n;
