@@ -411,13 +411,16 @@ __global__ __launch_bounds__(NW * 64, 2) void k_kv_many(KvPages p, KvSeqs b, KvR
                 c = fmaxf(c, 1e-37f);                        // -inf * c stays -inf at a scale of zero
                 float mx = ninf();
                 if (masked) {
-                    const uint32_t bad0 = L.bad[turn][0], bad1 = L.bad[turn][1];
+                    // (the lane's half taken out first, so that what is compared with is constant:
+                    // it would be kept in 64 registers through the whole loop)
+                    const uint32_t bad0 = L.bad[turn][0] >> (h * 4), bad1 = L.bad[turn][1] >> (h * 4);
+                    const int left = lim - key - h * 4;
 #pragma unroll
                     for (int t = 0; t < 2; t++)
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            const int k = (i >> 2) * 8 + h * 4 + (i & 3);
-                            const bool in = key + t * 32 + k < lim && !(hole >> (2 * t + (i >> 3)) & 1);
+                            const int k = (i >> 2) * 8 + (i & 3);
+                            const bool in = t * 32 + k < left && !(hole >> (2 * t + (i >> 3)) & 1);
                             if (in && ((t ? bad1 : bad0) >> k & 1)) l = __builtin_nanf("");
                             st[t][i] = in ? st[t][i] : ninf();
                         }
