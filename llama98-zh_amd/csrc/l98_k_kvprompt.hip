@@ -11,10 +11,12 @@
 // each 16.
 //
 // Q8 goes through fp16: q scaled per row by a power of two (exact for bf16), K
-// and V as code * scale * 2^(6 - E) with E of the tile's largest scale (K) and
-// of the largest so far (V; the sums are rescaled when it grows), two roundings
-// of 2^-11 against the output's 2^-8; numbers below 2^-27 of the largest lose
-// bits.  bf16 caches are used as they are.  Weights are rounded to the same 16
+// and V as code * scale * 2^(-9 - E) with E of the tile's largest scale (K) and
+// of the largest so far (V; the sums are rescaled when it grows): a byte u in
+// an fp16's low bits is the subnormal u 2^-24, and one packed fma, u 2^-24 * f -
+// f 2^-17 with f the scale times 2^(15 - E) rounded to fp16, makes the number
+// of it.  Two roundings of 2^-11, against the output's 2^-8; numbers below
+// 2^-12 of the largest are held with a step of 2^-22 of it.  bf16 caches are used as they are.  Weights are rounded to the same 16
 // bits, and their sum, in fp32, is of the rounded ones.
 //
 // The running maximum is raised only where a tile exceeds it by 2^8 (weights
@@ -38,11 +40,10 @@ __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {   // packed fp16 product
-    f16x2 x, y;
+__device__ __forceinline__ uint32_t times_2m17(uint32_t a) {         // of two fp16
+    f16x2 x;
     __builtin_memcpy(&x, &a, 4);
-    __builtin_memcpy(&y, &b, 4);
-    x = x * y;
+    x = x * (f16x2){(_Float16)-0x1p-17f, (_Float16)-0x1p-17f};
     uint32_t r;
     __builtin_memcpy(&r, &x, 4);
     return r;
@@ -51,24 +52,6 @@ __device__ __forceinline__ float finite_or_0(float x) {
     return (u_from_f(x) & 0x7F800000u) == 0x7F800000u ? 0.0f : x;
 }
 __device__ __forceinline__ int exp_above(uint32_t bits) { return (int)(bits >> 23) - 126; }   // 2^this > the float >= 0
-// the wave's largest of each half of x, in both halves of the result: by DPP, over rows of 16, then over the rows
-__device__ __forceinline__ uint32_t wave_max2(uint32_t x) {
-    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-    auto step = [&](uint32_t y) {
-        u16x2 p, q;
-        __builtin_memcpy(&p, &x, 4);
-        __builtin_memcpy(&q, &y, 4);
-        p = __builtin_elementwise_max(p, q);
-        __builtin_memcpy(&x, &p, 4);
-    };
-    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, true));   // row_shr:1
-    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, true));
-    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, true));
-    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, true));
-    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, true));   // row_bcast:15 into rows 1, 3
-    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, true));   // row_bcast:31 into rows 2, 3
-    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
-}
 // c + the two fp16 or bf16 numbers of x
 template <class E> __device__ __forceinline__ float add2(uint32_t x, float c);
 template <> __device__ __forceinline__ float add2<_Float16>(uint32_t x, float c) {
@@ -97,57 +80,69 @@ struct Stage {
     uint32_t v[VU][4][ES];
     float ks[Q8 ? KU : 1][2];
     f32x4 vs[Q8 ? VU : 1][SG];
-    f32x4 kall, vall;                                        // this lane's share of all the tile's scales
-    uint32_t hole;                                           // bit i: keys 16 i .. of the tile have no page
+    f32x4 both[2];                                           // this lane's share of all the tile's scales
 };
 
-// The pages of a tile's four 16-key quarters (uniform: scalar loads).
-struct ManyPages {
-    int id[4];
-    uint32_t hole;
+// The pages of a tile's four 16-key quarters (uniform: scalar loads), as the
+// table has them; checked where they are used, a turn later, so that nothing
+// waits for them.  ONE: a tile lies within a page (pages of 64 rows and more).
+template <bool ONE>
+struct ManyIds {
+    int id[ONE ? 1 : 4];
 };
-__device__ __forceinline__ ManyPages many_pages(const KvPages &p, const int *table, int pages, int key) {
-    ManyPages x;
-    x.hole = 0;
+template <bool ONE>
+__device__ __forceinline__ ManyIds<ONE> many_ids(const KvPages &p, const int *table, int pages, int key) {
+    ManyIds<ONE> x;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int at = (key + 16 * i) >> p.shift, id = at < pages ? table[at] : -1;
-        const bool there = (unsigned)id < (unsigned)p.n_pages;
-        if (!there) x.hole |= 1u << i;
-        x.id[i] = there ? id : 0;
+    for (int i = 0; i < (ONE ? 1 : 4); i++) {
+        const int at = (key + 16 * i) >> p.shift;
+        x.id[i] = table[at < pages ? at : pages - 1];        // (a quarter behind the table is masked by the length)
     }
     return x;
 }
+template <bool ONE>
+struct ManyPages {
+    uint32_t id[ONE ? 1 : 4];
+    uint32_t hole;                                           // bit i: keys 16 i .. of the tile have no page
+};
+template <bool ONE>
+__device__ __forceinline__ ManyPages<ONE> many_pages(const KvPages &p, const ManyIds<ONE> &t) {
+    ManyPages<ONE> x;
+    x.hole = 0;
+#pragma unroll
+    for (int i = 0; i < (ONE ? 1 : 4); i++) {
+        const bool there = (unsigned)t.id[i] < (unsigned)p.n_pages;
+        if (!there) x.hole |= ONE ? 15u : 1u << i;
+        x.id[i] = there ? (uint32_t)t.id[i] : 0u;
+    }
+    return x;
+}
+// Where the tile's key k (the thread's own) has something that lies `lane`
+// bytes into the page's block for key 0 and `step` bytes further for each key.
+// ONE: a uniform address and the thread's constant offset.
+template <bool ONE>
+__device__ __forceinline__ const unsigned char *many_at(const KvPages &p, const ManyPages<ONE> &pg, int key, uint32_t k,
+                                                        uint32_t lane, uint32_t step) {
+    const uint32_t unit = (uint32_t)(p.page_bytes >> 4), rows = 1u << p.shift, at0 = (uint32_t)key & (rows - 1);
+    if (ONE) return p.data + (((uint64_t)pg.id[0] * unit) << 4) + (uint64_t)(at0 * step) + (lane + k * step);
+    const uint32_t id0 = pg.id[0], id1 = pg.id[ONE ? 0 : 1], id2 = pg.id[ONE ? 0 : 2], id3 = pg.id[ONE ? 0 : 3];
+    const uint32_t a = k & 16 ? id1 : id0, c = k & 16 ? id3 : id2, id = k & 32 ? c : a;
+    return p.data + (((uint64_t)id * unit) << 4) + (lane + ((at0 + k) & (rows - 1)) * step);
+}
 
-template <int D, bool Q8, int NT>
-__device__ __forceinline__ void many_load(Stage<D, Q8, NT> &S, const KvPages &p, const ManyPages &pg, int kh, int key) {
+template <int D, bool Q8, int NT, bool ONE>
+__device__ __forceinline__ void many_load(Stage<D, Q8, NT> &S, const KvPages &p, const ManyPages<ONE> &pg, int kh, int key) {
     using T = Stage<D, Q8, NT>;
-    const uint32_t rows = 1u << p.shift, vo = (uint32_t)p.hk << p.shift, tid = threadIdx.x, at0 = (uint32_t)key & (rows - 1);
-    const uint32_t unit = (uint32_t)(p.page_bytes >> 4), scales = 2 * vo * D, head = (uint32_t)kh << p.shift;
-    S.hole = pg.hole;
-    const uint32_t id0 = pg.id[0], id1 = pg.id[1], id2 = pg.id[2], id3 = pg.id[3];
-    auto page = [=](uint32_t k) {                            // of the tile's key k
-        const uint32_t a = k & 16 ? id1 : id0, c = k & 16 ? id3 : id2, id = k & 32 ? c : a;
-        return p.data + (((uint64_t)id * unit) << 4);
-    };
-    auto row = [&](uint32_t k) { return (at0 + k) & (rows - 1); };
+    const uint32_t tid = threadIdx.x, head = ((uint32_t)kh << p.shift) * (D * T::ES), vo = ((uint32_t)p.hk << p.shift) * (D * T::ES);
 #pragma unroll
     for (int u = 0; u < T::KU; u++) {
         const uint32_t x = u * NT + tid, k = x / T::KROW % MANY_KEYS, c = x % T::KROW;
-        const unsigned char *pk = page(k);
-        S.k[u] = *(const u32x4 *)(pk + ((head + row(k)) * (D * T::ES) + c * 16));
-        if (Q8) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const uint32_t g = (2 * c + i) % T::G;       // chunk h G + g holds 8 numbers of group g
-                S.ks[u][i] = *(const float *)(pk + (scales + (((kh * T::G + g) << p.shift) + row(k)) * 4));
-            }
-        }
+        S.k[u] = *(const u32x4 *)many_at<ONE>(p, pg, key, k, head + c * 16, D * T::ES);
     }
 #pragma unroll
     for (int u = 0; u < T::VU; u++) {
         const uint32_t x = u * NT + tid, k = x / T::VROW * 4 % MANY_KEYS, c = x % T::VROW;
-        const unsigned char *pv = page(k), *s = pv + ((vo + head + row(k)) * (D * T::ES) + c * 4 * T::ES);
+        const unsigned char *s = many_at<ONE>(p, pg, key, k, vo + head + c * 4 * T::ES, D * T::ES);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             if (Q8) {
@@ -158,39 +153,78 @@ __device__ __forceinline__ void many_load(Stage<D, Q8, NT> &S, const KvPages &p,
                 S.v[u][i][T::ES - 1] = y.y;
             }
         }
-        if (Q8) {
-            const uint32_t g = D == 32 ? 0 : (4 * c) % (D / 16) / 2;         // byte n (D/16) + t: group t / 2
+    }
+}
+
+// The Q8 scales of the tile that S holds: the thread's own, and its share of
+// all of them (every wave over all of the tile's, so that all know the same
+// exponents: lanes 0-31 K's, 32-63 V's).
+template <int D, bool Q8, int NT, bool ONE>
+__device__ __forceinline__ void many_scales(Stage<D, Q8, NT> &S, const KvPages &p, const ManyPages<ONE> &pg, int kh, int key) {
+    using T = Stage<D, Q8, NT>;
+    if (!Q8) return;
+    const uint32_t tid = threadIdx.x, scales = 2 * ((uint32_t)p.hk << p.shift) * D;
+    // group g: of K kh G + g, of V behind all of K's
+    auto scale = [&](uint32_t g, uint32_t k) { return many_at<ONE>(p, pg, key, k, scales + (g << p.shift) * 4, 4); };
 #pragma unroll
-            for (int i = 0; i < T::SG; i++)
-                S.vs[u][i] = *(const f32x4 *)(pv + (scales + ((((p.hk + kh) * T::G + g + i) << p.shift) + row(k)) * 4));
-        }
+    for (int u = 0; u < T::KU; u++) {
+        const uint32_t x = u * NT + tid, k = x / T::KROW % MANY_KEYS, c = x % T::KROW;
+        // chunk h G + g holds 8 numbers of group g
+#pragma unroll
+        for (int i = 0; i < 2; i++) S.ks[u][i] = *(const float *)scale(kh * T::G + (2 * c + i) % T::G, k);
     }
-    if (Q8) {
-        // every wave over all of the tile's scales, so that all know the same exponents
-        const uint32_t lane = tid & 63, k = (lane & 15) * 4, g = (lane >> 4) % T::G;
-        const unsigned char *s = page(k) + (scales + (((kh * T::G + g) << p.shift) + row(k)) * 4);
-        S.kall = *(const f32x4 *)s;
-        S.vall = *(const f32x4 *)(s + (vo * T::G) * 4);
+#pragma unroll
+    for (int u = 0; u < T::VU; u++) {
+        const uint32_t x = u * NT + tid, k = x / T::VROW * 4 % MANY_KEYS, c = x % T::VROW;
+        const uint32_t g = D == 32 ? 0 : (4 * c) % (D / 16) / 2;             // byte n (D/16) + t: group t / 2
+#pragma unroll
+        for (int i = 0; i < T::SG; i++) S.vs[u][i] = *(const f32x4 *)scale((p.hk + kh) * T::G + g + i, k);
     }
+    // 64 keys of G groups over 32 lanes, 8 of them each
+    const uint32_t lane = tid & 31, k = (lane & 7) * 8, g = (lane >> 3) % T::G + (tid & 32 ? p.hk + kh : kh) * T::G;
+    const unsigned char *s = scale(g, k);
+    S.both[0] = *(const f32x4 *)s;
+    S.both[1] = *(const f32x4 *)(s + 16);
 }
 
 // Exponents above the tile's K and V scales, of the keys that exist.
 template <int D, bool Q8, int NT>
-__device__ __forceinline__ void many_exps(Stage<D, Q8, NT> &S, int key, int len, bool masked, int &ek, int &ev) {
+__device__ __forceinline__ void many_exps(Stage<D, Q8, NT> &S, uint32_t hole, int key, int len, bool masked, int &ek, int &ev) {
     if (masked) {
-        const int k = (threadIdx.x & 15) * 4;
+        const int k = (threadIdx.x & 7) * 8;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const bool in = key + k + i < len && !(S.hole >> (k >> 4) & 1);
-            S.kall[i] = in ? finite_or_0(S.kall[i]) : 0.0f;
-            S.vall[i] = in ? finite_or_0(S.vall[i]) : 0.0f;
+        for (int i = 0; i < 8; i++) {
+            const bool in = key + k + i < len && !(hole >> (k >> 4) & 1);
+            S.both[i >> 2][i & 3] = in ? finite_or_0(S.both[i >> 2][i & 3]) : 0.0f;
         }
     }
-    const float a = fmaxf(fmaxf(S.kall[0], S.kall[1]), fmaxf(S.kall[2], S.kall[3]));
-    const float c = fmaxf(fmaxf(S.vall[0], S.vall[1]), fmaxf(S.vall[2], S.vall[3]));
-    const uint32_t x = wave_max2(__builtin_amdgcn_perm(u_from_f(a), u_from_f(c), 0x07060302u));
-    ek = exp_above(x & 0xFFFF0000u);
-    ev = exp_above(x << 16);
+    float a = fmaxf(S.both[0][0], S.both[0][1]);
+#pragma unroll
+    for (int i = 2; i < 8; i++) a = fmaxf(a, S.both[i >> 2][i & 3]);
+    // the largest of each 32 lanes, in the last of them: by DPP, over rows of 16, then into the odd rows
+    uint32_t x = u_from_f(a);
+    auto step = [&](uint32_t y) { x = y > x ? y : x; };
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, true));   // row_shr:1
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, true));
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, true));
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, true));
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, true));   // row_bcast:15 into rows 1, 3
+    ek = exp_above((uint32_t)__builtin_amdgcn_readlane((int)x, 31));
+    ev = exp_above((uint32_t)__builtin_amdgcn_readlane((int)x, 63));
+}
+
+// bytes of lo and hi (sel: a byte of each over zeros), each minus 128, times
+// the scales' halves of f = 2^15 times what they are multiplied with; c = -f / 2^17
+__device__ __forceinline__ uint32_t scaled2(uint32_t hi, uint32_t lo, uint32_t sel, uint32_t f, uint32_t c) {
+    const uint32_t u = __builtin_amdgcn_perm(hi, lo, sel);   // as fp16: subnormals, u 2^-24
+    f16x2 x, y, z;
+    __builtin_memcpy(&x, &u, 4);
+    __builtin_memcpy(&y, &f, 4);
+    __builtin_memcpy(&z, &c, 4);
+    x = __builtin_elementwise_fma(x, y, z);
+    uint32_t r;
+    __builtin_memcpy(&r, &x, 4);
+    return r;
 }
 
 // 16-byte chunk c of row r (of CH chunks) in LDS: rows of less than 256 bytes
@@ -202,13 +236,13 @@ __device__ __forceinline__ int chunk_at(int r, int c) {
 
 template <int D>
 struct ManyLds {
-    uint16_t k[2][MANY_KEYS * D], v[2][MANY_KEYS * D];
-    uint32_t bad[3][2];                                      // keys of a masked tile whose V is not finite, by tile % 3
+    uint16_t k[2][MANY_KEYS * D], v[3][MANY_KEYS * D];       // of tile % 2, % 3
+    uint32_t bad[4][2];                                      // keys of a masked tile whose V is not finite, by tile % 4
 };
 
 template <int D, bool Q8, int NT>
-__device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, ManyLds<D> &L, int buf, int turn, int key, int len, bool masked,
-                                           int ek, int ev) {
+__device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, ManyLds<D> &L, uint32_t holes, int kb, int vb, int fb,
+                                           int key, int len, bool masked, int ek, int ev) {
     using T = Stage<D, Q8, NT>;
     const int tid = threadIdx.x;
 #pragma unroll
@@ -219,18 +253,18 @@ __device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, ManyLds<D> &L, i
         if (Q8) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float f = __builtin_amdgcn_ldexpf(S.ks[u][i], 15 - ek);
-                const uint32_t ff = pack2<_Float16>(f, f);
+                const float x = __builtin_amdgcn_ldexpf(S.ks[u][i], 15 - ek);
+                const uint32_t f = pack2<_Float16>(x, x), c2 = times_2m17(f);
                 u32x4 o;
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
-                    o[2 * w] = mul2(codes2(0, S.k[u][2 * i + w], 0x0c010c00u), ff);
-                    o[2 * w + 1] = mul2(codes2(0, S.k[u][2 * i + w], 0x0c030c02u), ff);
+                    o[2 * w] = scaled2(0, S.k[u][2 * i + w], 0x0c010c00u, f, c2);
+                    o[2 * w + 1] = scaled2(0, S.k[u][2 * i + w], 0x0c030c02u, f, c2);
                 }
-                *(u32x4 *)&L.k[buf][chunk_at<D / 8>(k, 2 * c + i) * 8] = o;
+                *(u32x4 *)&L.k[kb][chunk_at<D / 8>(k, 2 * c + i) * 8] = o;
             }
         } else {
-            *(u32x4 *)&L.k[buf][chunk_at<D / 8>(k, c) * 8] = S.k[u];
+            *(u32x4 *)&L.k[kb][chunk_at<D / 8>(k, c) * 8] = S.k[u];
         }
     }
 #pragma unroll
@@ -239,7 +273,7 @@ __device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, ManyLds<D> &L, i
         if (T::VT % NT && x >= T::VT) break;
         const int k = x / T::VROW * 4, c = x % T::VROW;
         if (masked) {
-            const bool hole = S.hole >> (k >> 4) & 1;
+            const bool hole = holes >> (k >> 4) & 1;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 bool bad = false;
@@ -256,19 +290,21 @@ __device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, ManyLds<D> &L, i
 #pragma unroll
                     for (int w = 0; w < T::ES; w++) S.v[u][i][w] = gone || bad ? 0u : S.v[u][i][w];
                 }
-                if (bad && !gone) atomicOr(&L.bad[turn][(k + i) >> 5], 1u << ((k + i) & 31));
+                if (bad && !gone) atomicOr(&L.bad[fb][(k + i) >> 5], 1u << ((k + i) & 31));
             }
         }
         // the quad's place: 0-3, 8-11, 4-7, 12-15 of each 16 keys
         const int r = (k >> 2) & 3, slot = (k >> 4) * 16 + ((r & 1) * 2 + (r >> 1)) * 4;
-        uint32_t f[T::SG][2];
+        uint32_t f[T::SG][2], f2[T::SG][2];
         if (Q8) {
 #pragma unroll
             for (int g = 0; g < T::SG; g++)
 #pragma unroll
-                for (int w = 0; w < 2; w++)
+                for (int w = 0; w < 2; w++) {
                     f[g][w] = pack2<_Float16>(__builtin_amdgcn_ldexpf(S.vs[u][g][2 * w], 15 - ev),
                                               __builtin_amdgcn_ldexpf(S.vs[u][g][2 * w + 1], 15 - ev));
+                    f2[g][w] = times_2m17(f[g][w]);
+                }
         }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -279,8 +315,8 @@ __device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, ManyLds<D> &L, i
                 dim = pos % (D / 16) * 16 + pos / (D / 16);
                 const int g = T::SG == 1 ? 0 : e >> 1;
                 const uint32_t sel = 0x0c040c00u + (uint32_t)e * 0x00010001u;
-                o.x = mul2(codes2(S.v[u][1][0], S.v[u][0][0], sel), f[g][0]);
-                o.y = mul2(codes2(S.v[u][3][0], S.v[u][2][0], sel), f[g][1]);
+                o.x = scaled2(S.v[u][1][0], S.v[u][0][0], sel, f[g][0], f2[g][0]);
+                o.y = scaled2(S.v[u][3][0], S.v[u][2][0], sel, f[g][1], f2[g][1]);
             } else {
                 dim = pos;
                 const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
@@ -288,13 +324,13 @@ __device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, ManyLds<D> &L, i
                 o.x = __builtin_amdgcn_perm(S.v[u][1][e >> 1 ? H : 0], S.v[u][0][e >> 1 ? H : 0], sel);
                 o.y = __builtin_amdgcn_perm(S.v[u][3][e >> 1 ? H : 0], S.v[u][2][e >> 1 ? H : 0], sel);
             }
-            *(uint2 *)&L.v[buf][chunk_at<8>(dim, slot >> 3) * 8 + (slot & 7)] = o;
+            *(uint2 *)&L.v[vb][chunk_at<8>(dim, slot >> 3) * 8 + (slot & 7)] = o;
         }
     }
 }
 
-template <int D, bool Q8, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void k_kv_many(KvPages p, KvSeqs b, KvRows q, KvRows out, int heads, int group,
+template <int D, bool Q8, int NW, bool ONE>
+__global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_many(KvPages p, KvSeqs b, KvRows q, KvRows out, int heads, int group,
                                                         float scale2, int chunk, int tiles, int vec, KvParts w) {
     using E = typename std::conditional<Q8, _Float16, __bf16>::type;
     using V8 = typename std::conditional<Q8, f16x8, bf16x8>::type;
@@ -313,10 +349,9 @@ __global__ __launch_bounds__(NW * 64, 2) void k_kv_many(KvPages p, KvSeqs b, KvR
         return e < s.len ? e : s.len;
     };
     const int k0 = split * chunk;
-    int k1 = k0 + chunk, wend = end_of(tile * ROWS + wave * 32 + 31);
+    int k1 = k0 + chunk;
     const int end = end_of(tile * ROWS + ROWS - 1), all = end_of(tile * ROWS);
     k1 = k1 < end ? k1 : end;
-    wend = wend < k1 ? wend : k1;
     const int *table = b.table + seq * b.stride;
 
     const int row = tile * ROWS + wave * 32 + n, j = row / group, head = kh * group + row % group, r = s.r0 + j;
@@ -352,83 +387,160 @@ __global__ __launch_bounds__(NW * 64, 2) void k_kv_many(KvPages p, KvSeqs b, KvR
             const uint32_t o = __shfl_xor(big, 32);
             big = o > big ? o : big;
             e = (int)(big >> 23) - 127 - 14;
-            cq = __builtin_amdgcn_ldexpf(cq, e - 6);         // K comes with 2^(6 - ek)
+            cq = __builtin_amdgcn_ldexpf(cq, e + 9);         // K comes with 2^(-9 - ek)
         }
 #pragma unroll
         for (int c = 0; c < KK; c++)
 #pragma unroll
             for (int i = 0; i < 8; i++) qf[c][i] = (E)(Q8 ? __builtin_amdgcn_ldexpf(x[c][i], -e) : x[c][i]);
     }
-    f32x16 o[DT] = {};
+    f32x16 o[DT] = {}, st[2];
+    u32x4 pw[2][2] = {};                                     // weights of the tile before
     float m = ninf(), l = 0.0f;
-    int ek = 0, ev = -1000;                                  // exponents of the tile in LDS
+    int ev = -1000;                                          // the unit's exponent of the sums
 
     if (k0 < k1) {
-        if (threadIdx.x < 6) L.bad[threadIdx.x >> 1][threadIdx.x & 1] = 0;
+        // Two halves of the block's waves, one of each on every SIMD, take turns:
+        // while one has the matrix cores (the values of tile i - 1, the scores of
+        // tile i), the other does tile i's softmax and brings the next tile
+        // into LDS, a barrier between the turns.  With slots of time counted
+        // from 0, half g has the matrix cores for tile i in slot 2 i + g.  Its
+        // share of tile i + 1 + g is stored in the slot after that, so tile j is
+        // stored in slots 2 j - 2 and 2 j - 1: its K is read in slots 2 j and
+        // 2 j + 1, its V in 2 j + 2 and 2 j + 3, and with two buffers for K and
+        // three for V nothing is overwritten before its last reader's slot ends.
+        const int g = wave / (NW / 2), n_tiles = (k1 - k0 + MANY_KEYS - 1) / MANY_KEYS;
+        // of a stored tile, all uniform: the exponents, and its holes | 16 if it is
+        // masked; of tile i, of tile i + 1 (in half 1), of the one just stored
+        int ek0 = 0, ev0 = 0, ek1 = 0, ev1 = 0, ek2 = 0, ev2 = 0;
+        uint32_t how0 = 0, how1 = 0, how2 = 0;
+        if (threadIdx.x < 8) L.bad[threadIdx.x >> 1][threadIdx.x & 1] = 0;
+        // the first turn's values are of a tile that is not: no weights, and numbers to take them times
+        for (int x = threadIdx.x; x < MANY_KEYS * D / 8; x += NT) ((u32x4 *)L.v[2])[x] = u32x4{0, 0, 0, 0};
         __syncthreads();
-        int evn = ev, ekn = 0;
-        auto bounds = [&](Stage<D, Q8, NT> &S, int key, bool masked) {
-            if (!Q8) return;
-            int x;
-            many_exps<D, Q8, NT>(S, key, s.len, masked, ekn, x);
-            evn = evn > x ? evn : x;
-        };
+        int eb = -1000;                                      // V's exponent so far
+        auto at = [&](int i) { return k0 + (i < n_tiles ? i : n_tiles - 1) * MANY_KEYS; };
         Stage<D, Q8, NT> S;
-        ManyPages pg = many_pages(p, table, b.pages, k0);
-        bool masked = k0 + MANY_KEYS > all || pg.hole, next_masked;
-        many_load<D, Q8, NT>(S, p, pg, kh, k0);
-        uint32_t hole = S.hole;
-        bounds(S, k0, masked);
-        many_store<D, Q8, NT>(S, L, 0, 0, k0, s.len, masked, ekn, evn);
-        pg = many_pages(p, table, b.pages, k0 + MANY_KEYS < k1 ? k0 + MANY_KEYS : k0);
-        __syncthreads();
-        for (int key = k0, buf = 0, turn = 0; key < k1; key += MANY_KEYS, buf ^= 1) {
-            const int next = key + MANY_KEYS, turn1 = turn == 2 ? 0 : turn + 1;
-            // the flags of the tile before this one, which nobody reads or sets in this turn
-            if (threadIdx.x < 2) L.bad[turn == 0 ? 2 : turn - 1][threadIdx.x] = 0;
-            if (Q8 && evn != ev) {                           // the V scales' unit grew
-                if (ev != -1000) {
-                    const float f = __builtin_amdgcn_ldexpf(1.0f, ev - evn);
-#pragma unroll
-                    for (int d = 0; d < DT; d++) o[d] *= f;
-                }
-                ev = evn;
+        ManyPages<ONE> pg;                                        // of the tile in S
+        ManyIds<ONE> next = many_ids<ONE>(p, table, b.pages, at(0));  // of the one behind it
+        auto load = [&](int i) {                             // tile i (the last one again behind the end)
+            pg = many_pages<ONE>(p, next);
+            many_load<D, Q8, NT, ONE>(S, p, pg, kh, at(i));
+            next = many_ids<ONE>(p, table, b.pages, at(i + 1));
+        };
+        auto store = [&](int i) {
+            const int key = at(i);
+            const bool masked = key + MANY_KEYS > all || pg.hole;
+            how2 = pg.hole | (masked ? 16u : 0u);
+            if (Q8) {
+                int e;
+                many_exps<D, Q8, NT>(S, pg.hole, key, s.len, masked, ek2, e);
+                eb = eb > e ? eb : e;
+                ev2 = eb;
             }
-            ek = ekn;
-            // (the last turn loads its own tile again, without a branch)
-            many_load<D, Q8, NT>(S, p, pg, kh, next < k1 ? next : key);
-            pg = many_pages(p, table, b.pages, next + MANY_KEYS < k1 ? next + MANY_KEYS : key);
-            if (key < wend) {
-                f32x16 st[2] = {};
+            if (i < n_tiles) many_store<D, Q8, NT>(S, L, pg.hole, i & 1, i % 3, i & 3, key, s.len, masked, ek2, ev2);
+        };
+        load(0);
+        many_scales<D, Q8, NT, ONE>(S, p, pg, kh, at(0));
+        store(0);
+        ek0 = ek2;
+        ev0 = ev2;
+        how0 = how2;
+        load(1);
+        if (g) {
+            many_scales<D, Q8, NT, ONE>(S, p, pg, kh, at(1));
+            store(1);
+            ek1 = ek2;
+            ev1 = ev2;
+            how1 = how2;
+            load(2);
+        }
+        __syncthreads();
+        if (g) __syncthreads();
+        // The fragments of a turn: 4 DT of V for the values of tile i - 1, then 2 KK
+        // of K for the scores of tile i, read in fours one four ahead of the
+        // instructions that take them.  The scheduling barriers keep it so: left
+        // to itself the compiler reads each where it is used, and waits for it.
+        constexpr int NV = 4 * DT, NF = NV + 2 * KK;
+        // byte addresses of the lane's row and first chunk; a fragment's own chunk
+        // is an exclusive or away (chunk_at), its row a multiple of 32
+        const uint32_t lane_v = chunk_at<8>(n, h) * 16, lane_k = chunk_at<D / 8>(n, h) * 16;
+        uint32_t row_v = 0, row_k = 0;
+        auto fragment = [&](int x) {
+            if (x < NV) return *(const u32x4 *)((const char *)L.v[0] + (row_v ^ (uint32_t)(x / DT << 5)) + x % DT * (32 * 128));
+            x -= NV;
+            return *(const u32x4 *)((const char *)L.k[0] + (row_k ^ (uint32_t)(x / 2 << 5)) + x % 2 * (32 * 2 * D));
+        };
+        auto product = [&](int x, const u32x4 &f) {
+            if (x < NV) {
+                o[x % DT] = mfma32(as<V8>(f), as<V8>(pw[x / DT / 2][x / DT % 2]), o[x % DT]);
+            } else {
+                x -= NV;
+                st[x % 2] = mfma32(as<V8>(f), qf[x / 2], st[x % 2]);
+            }
+        };
+        auto turn = [&](auto first, auto behind, int i) {
+            constexpr int A = decltype(first)::value, B = decltype(behind)::value;
+            u32x4 f[2][4];
+            row_v = lane_v + (i + 2) % 3 * (uint32_t)sizeof(L.v[0]);
+            row_k = lane_k + (i & 1) * (uint32_t)sizeof(L.k[0]);
+            if (B == NF) {
+                st[0] = f32x16{};
+                st[1] = f32x16{};
+            }
 #pragma unroll
-                for (int c = 0; c < KK; c++)
+            for (int e = 0; e < 4; e++) f[0][e] = fragment(A + e);
 #pragma unroll
-                    for (int t = 0; t < 2; t++) {
-                        const u32x4 a = *(const u32x4 *)&L.k[buf][chunk_at<D / 8>(t * 32 + n, 2 * c + h) * 8];
-                        st[t] = mfma32(as<V8>(a), qf[c], st[t]);
+            for (int x = A; x < B; x += 4) {
+                if (x + 4 < B)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) f[(x - A) / 4 + 1 & 1][e] = fragment(x + 4 + e);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int e = 0; e < 4; e++) product(x + e, f[(x - A) / 4 & 1][e]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        typedef std::integral_constant<int, 0> c0;
+        typedef std::integral_constant<int, NV> cv;
+        typedef std::integral_constant<int, NF> cf;
+        for (int i = 0; i < n_tiles; i++) {
+            const int key = k0 + i * MANY_KEYS;
+            turn(c0(), cf(), i);
+            __syncthreads();
+            // (not with the tile's codes: they would take registers through the turn)
+            many_scales<D, Q8, NT, ONE>(S, p, pg, kh, at(i + 1 + g));
+            {
+                if (Q8 && ev0 != ev) {                       // the V scales' unit grew
+                    if (ev != -1000) {
+                        const float f = __builtin_amdgcn_ldexpf(1.0f, ev - ev0);
+#pragma unroll
+                        for (int d = 0; d < DT; d++) o[d] *= f;
                     }
-                float c = Q8 ? __builtin_amdgcn_ldexpf(cq, ek) : cq;
+                    ev = ev0;
+                }
+                float c = Q8 ? __builtin_amdgcn_ldexpf(cq, ek0) : cq;
                 c = fmaxf(c, 1e-37f);                        // -inf * c stays -inf at a scale of zero
                 float mx = ninf();
-                if (masked) {
+                if (how0 & 16u) {
                     // (the lane's half taken out first, so that what is compared with is constant:
                     // it would be kept in 64 registers through the whole loop)
-                    const uint32_t bad0 = L.bad[turn][0] >> (h * 4), bad1 = L.bad[turn][1] >> (h * 4);
+                    const uint32_t bad0 = L.bad[i & 3][0] >> (h * 4), bad1 = L.bad[i & 3][1] >> (h * 4);
                     const int left = lim - key - h * 4;
 #pragma unroll
                     for (int t = 0; t < 2; t++)
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const int k = (i >> 2) * 8 + (i & 3);
-                            const bool in = t * 32 + k < left && !(hole >> (2 * t + (i >> 3)) & 1);
+                        for (int e = 0; e < 16; e++) {
+                            const int k = (e >> 2) * 8 + (e & 3);
+                            const bool in = t * 32 + k < left && !(how0 >> (2 * t + (e >> 3)) & 1);
                             if (in && ((t ? bad1 : bad0) >> k & 1)) l = __builtin_nanf("");
-                            st[t][i] = in ? st[t][i] : ninf();
+                            st[t][e] = in ? st[t][e] : ninf();
                         }
                 }
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++) mx = fmaxf(mx, st[t][i]);
+                    for (int e = 0; e < 16; e++) mx = fmaxf(mx, st[t][e]);
                 mx = fmaxf(mx, __shfl_xor(mx, 32)) * c;
                 // each row by itself: its bits must not depend on the wave's other rows
                 const bool up = mx > m + 8.0f;
@@ -443,41 +555,34 @@ __global__ __launch_bounds__(NW * 64, 2) void k_kv_many(KvPages p, KvSeqs b, KvR
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        st[t][i] = kv_exp2(__builtin_fmaf(st[t][i], c, -mu));
-                    }
+                    for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        u32x4 pw;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            pw[i] = pack2<E>(st[t][u * 8 + 2 * i], st[t][u * 8 + 2 * i + 1]);
-                            l = add2<E>(pw[i], l);
+                        for (int e = 0; e < 4; e++) {
+                            const float a = kv_exp2(__builtin_fmaf(st[t][u * 8 + 2 * e], c, -mu));
+                            const float d = kv_exp2(__builtin_fmaf(st[t][u * 8 + 2 * e + 1], c, -mu));
+                            pw[t][u][e] = pack2<E>(a, d);
+                            l = add2<E>(pw[t][u][e], l);
                         }
-#pragma unroll
-                        for (int d = 0; d < DT; d++) {
-                            const u32x4 a = *(const u32x4 *)&L.v[buf][chunk_at<8>(d * 32 + n, (t * 2 + u) * 2 + h) * 8];
-                            o[d] = mfma32(as<V8>(a), as<V8>(pw), o[d]);
-                        }
-                    }
             }
-            if (next < k1) {
-                hole = S.hole;
-                next_masked = next + MANY_KEYS > all || hole;
-                bounds(S, next, next_masked);
-                many_store<D, Q8, NT>(S, L, buf ^ 1, turn1, next, s.len, next_masked, ekn, evn);
-                masked = next_masked;
-            }
-            turn = turn1;
+            // the flags of the tile before this one, which nobody reads or sets in this slot
+            if (!g && threadIdx.x < 2) L.bad[(i + 3) & 3][threadIdx.x] = 0;
+            store(i + 1 + g);
+            load(i + 2 + g);
+            ek0 = g ? ek1 : ek2;
+            ev0 = g ? ev1 : ev2;
+            how0 = g ? how1 : how2;
+            ek1 = ek2;
+            ev1 = ev2;
+            how1 = how2;
             __syncthreads();
         }
+        if (!g) __syncthreads();
+        turn(c0(), cv(), n_tiles);
     }
     l += __shfl_xor(l, 32);
     if (!on) return;
     if (Q8) {
-        const float f = __builtin_amdgcn_ldexpf(1.0f, ev == -1000 ? 0 : ev - 6);
+        const float f = __builtin_amdgcn_ldexpf(1.0f, ev == -1000 ? 0 : ev + 9);
 #pragma unroll
         for (int d = 0; d < DT; d++) o[d] *= f;
     }
@@ -526,12 +631,17 @@ static int many(const KvPages &p, const KvSeqs &b, const KvRows &q, const KvRows
                 const KvPlan &x, const KvParts &w, hipStream_t st) {
     const int vec = aligned16(q) && aligned16(o);
     const dim3 grid((unsigned)((long long)x.splits * p.hk * x.tiles), b.n_seq);
-    if (x.rows == 128)
-        hipLaunchKernelGGL((k_kv_many<D, Q8, 4>), grid, dim3(256), 0, st, p, b, q, o, heads, heads / p.hk, scale2, x.chunk,
-                           x.tiles, vec, w);
-    else
-        hipLaunchKernelGGL((k_kv_many<D, Q8, 8>), grid, dim3(512), 0, st, p, b, q, o, heads, heads / p.hk, scale2, x.chunk,
-                           x.tiles, vec, w);
+#define MANY_LAUNCH(NW, ONE)                                                                                      \
+    hipLaunchKernelGGL((k_kv_many<D, Q8, NW, ONE>), grid, dim3(NW * 64), 0, st, p, b, q, o, heads, heads / p.hk,  \
+                       scale2, x.chunk, x.tiles, vec, w)
+    const bool one = (1 << p.shift) >= MANY_KEYS;
+    if (x.rows == 128) {
+        if (one) MANY_LAUNCH(4, true);
+        else MANY_LAUNCH(4, false);
+    } else {
+        if (one) MANY_LAUNCH(8, true);
+        else MANY_LAUNCH(8, false);
+    }
     return (int)hipGetLastError();
 }
 
