@@ -446,14 +446,13 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
         ek0 = ek2;
         ev0 = ev2;
         how0 = how2;
-        load(1);
         if (g) {
+            load(1);
             many_scales<D, Q8, NT, ONE>(S, p, pg, kh, at(1));
             store(1);
             ek1 = ek2;
             ev1 = ev2;
             how1 = how2;
-            load(2);
         }
         __syncthreads();
         if (g) __syncthreads();
@@ -479,7 +478,8 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
                 st[x % 2] = mfma32(as<V8>(f), qf[x / 2], st[x % 2]);
             }
         };
-        auto turn = [&](auto first, auto behind, int i) {
+        // `beside` is done while the matrix cores have the first four
+        auto turn = [&](auto first, auto behind, int i, auto beside) {
             constexpr int A = decltype(first)::value, B = decltype(behind)::value;
             u32x4 f[2][4];
             row_v = lane_v + (i + 2) % 3 * (uint32_t)sizeof(L.v[0]);
@@ -498,6 +498,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int e = 0; e < 4; e++) product(x + e, f[(x - A) / 4 & 1][e]);
+                if (x == A) beside();
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
@@ -506,10 +507,10 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
         typedef std::integral_constant<int, NF> cf;
         for (int i = 0; i < n_tiles; i++) {
             const int key = k0 + i * MANY_KEYS;
-            turn(c0(), cf(), i);
-            __syncthreads();
+            turn(c0(), cf(), i, [&]() { load(i + 1 + g); });
             // (not with the tile's codes: they would take registers through the turn)
             many_scales<D, Q8, NT, ONE>(S, p, pg, kh, at(i + 1 + g));
+            __syncthreads();
             {
                 if (Q8 && ev0 != ev) {                       // the V scales' unit grew
                     if (ev != -1000) {
@@ -567,7 +568,6 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
             // the flags of the tile before this one, which nobody reads or sets in this slot
             if (!g && threadIdx.x < 2) L.bad[(i + 3) & 3][threadIdx.x] = 0;
             store(i + 1 + g);
-            load(i + 2 + g);
             ek0 = g ? ek1 : ek2;
             ev0 = g ? ev1 : ev2;
             how0 = g ? how1 : how2;
@@ -577,7 +577,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
             __syncthreads();
         }
         if (!g) __syncthreads();
-        turn(c0(), cv(), n_tiles);
+        turn(c0(), cv(), n_tiles, []() {});
     }
     l += __shfl_xor(l, 32);
     if (!on) return;
