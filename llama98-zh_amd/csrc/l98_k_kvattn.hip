@@ -706,13 +706,13 @@ int attend(const KvPages &p, int q8, const KvSeqs &b, const KvRows &q, const KvR
     const KvPlan x = plan(p, b, heads, bf16);
     KvParts w;
     w.splits = x.splits;
-    w.o = (float *)ws;
+    w.o = (float *)((char *)ws + (x.many ? l98k_kv_many_ws(p, b) : 0));
     w.ml = w.o + (long long)b.n_rows * heads * x.splits * D;
     const float scale2 = scale * 1.44269504088896341f;
     const long long blocks = (long long)x.splits * p.hk * x.tiles, joins = (long long)b.max_rows * heads;
     if (blocks > INT_MAX || joins > INT_MAX) return -1;
     int rc;
-    if (x.many) rc = l98k_kv_many(p, q8, b, q, o, heads, scale2, x, w, st);
+    if (x.many) rc = l98k_kv_many(p, q8, b, q, o, heads, scale2, x, w, ws, st);
     else if (q8) rc = bf16 ? few<D, true, true>(p, b, q, o, heads, scale2, x, w, st)
                            : few<D, true, false>(p, b, q, o, heads, scale2, x, w, st);
     else rc = bf16 ? few<D, false, true>(p, b, q, o, heads, scale2, x, w, st)
@@ -727,7 +727,7 @@ int attend(const KvPages &p, int q8, const KvSeqs &b, const KvRows &q, const KvR
 
 extern "C" long long l98k_kv_attend_ws(const KvPages &p, int, const KvSeqs &b, int heads, int bf16) {
     const KvPlan x = plan(p, b, heads, bf16);
-    return x.splits == 1 ? 0 : (long long)b.n_rows * heads * x.splits * (p.d + 2) * 4;
+    return (x.many ? l98k_kv_many_ws(p, b) : 0) + (x.splits == 1 ? 0 : (long long)b.n_rows * heads * x.splits * (p.d + 2) * 4);
 }
 
 extern "C" int l98k_kv_attend(const KvPages &p, int q8, const KvSeqs &b, const KvRows &q, const KvRows &o, int heads,

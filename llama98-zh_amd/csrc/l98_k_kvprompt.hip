@@ -1,23 +1,30 @@
 // Causal attention of many new rows over the paged key-value cache, bf16 rows.
 //
-// The bound is the matrix cores: a block takes 32 NW rows of one (sequence, kv
-// head), 32 for each of its waves, and goes over the keys in tiles of 64 that
-// all waves share.  A tile comes from its pages into registers one tile ahead
-// and from there, converted, into one of two LDS buffers: K as [key][dim], V
-// transposed as [dim][key], 16-byte chunks permuted so that the fragments'
-// reads are free of bank conflicts.  S^T = K Q^T and O^T += V^T P^T by 32 x 32 x
-// 16 instructions: a lane's S^T (query lane & 31) is the second product's
-// operand as it stands, with V's keys in the order 0-3, 8-11, 4-7, 12-15 of
-// each 16.
+// Two launches.  k_kv_tiles turns each (sequence, kv head)'s keys into tiles of
+// 64 in the workspace, as the second one has them in LDS: K as [key][dim], V
+// transposed as [dim][key], in 16 bits, 16-byte chunks permuted so that the
+// fragments' reads are free of bank conflicts.  It reads the cache once and
+// writes 4 dim bytes per key, where each of the blocks below would convert all
+// of its keys again (a 16,384-token prompt, 4 kv heads of 128, Q8: 64 times;
+// with the conversion in the second kernel its waves issued 230 vector and 87
+// scalar instructions per tile beside the 32 matrix ones, and took 1.23 ms).
+//
+// k_kv_many: the bound is the matrix cores.  A block takes 32 NW rows of one
+// (sequence, kv head), 32 for each of its waves, and all waves share the tiles,
+// which are loaded straight into LDS two tiles ahead.  S^T = K Q^T and O^T += V^T
+// P^T by 32 x 32 x 16 instructions: a lane's S^T (query lane & 31) is the second
+// product's operand as it stands, with V's keys in the order 0-3, 8-11, 4-7,
+// 12-15 of each 16.
 //
 // Q8 goes through fp16: q scaled per row by a power of two (exact for bf16), K
-// and V as code * scale * 2^(-9 - E) with E of the tile's largest scale (K) and
-// of the largest so far (V; the sums are rescaled when it grows): a byte u in
-// an fp16's low bits is the subnormal u 2^-24, and one packed fma, u 2^-24 * f -
-// f 2^-17 with f the scale times 2^(15 - E) rounded to fp16, makes the number
-// of it.  Two roundings of 2^-11, against the output's 2^-8; numbers below
-// 2^-12 of the largest are held with a step of 2^-22 of it.  bf16 caches are used as they are.  Weights are rounded to the same 16
-// bits, and their sum, in fp32, is of the rounded ones.
+// and V as code * scale * 2^(-9 - E) with E of the tile's largest scale (the
+// sums are rescaled when a larger one of V's comes): a byte u in an fp16's low bits is the
+// subnormal u 2^-24, and one packed fma, u 2^-24 * f - f 2^-17 with f the scale
+// times 2^(15 - E) rounded to fp16, makes the number of it.  Two roundings of
+// 2^-11, against the output's 2^-8; numbers below 2^-12 of the tile's largest
+// are held with a step of 2^-22 of it.  bf16 caches are used as they are.
+// Weights are rounded to the same 16 bits, and their sum, in fp32, is of the
+// rounded ones.
 //
 // The running maximum is raised only where a tile exceeds it by 2^8 (weights
 // stay below 2^8): the sums are rescaled a few times per row instead of once
@@ -83,66 +90,46 @@ struct Stage {
     f32x4 both[2];                                           // this lane's share of all the tile's scales
 };
 
-// The pages of a tile's four 16-key quarters (uniform: scalar loads), as the
-// table has them; checked where they are used, a turn later, so that nothing
-// waits for them.  ONE: a tile lies within a page (pages of 64 rows and more).
-template <bool ONE>
-struct ManyIds {
-    int id[ONE ? 1 : 4];
-};
-template <bool ONE>
-__device__ __forceinline__ ManyIds<ONE> many_ids(const KvPages &p, const int *table, int pages, int key) {
-    ManyIds<ONE> x;
-#pragma unroll
-    for (int i = 0; i < (ONE ? 1 : 4); i++) {
-        const int at = (key + 16 * i) >> p.shift;
-        x.id[i] = table[at < pages ? at : pages - 1];        // (a quarter behind the table is masked by the length)
-    }
-    return x;
-}
-template <bool ONE>
+// The pages of a tile's four 16-key quarters (uniform).
 struct ManyPages {
-    uint32_t id[ONE ? 1 : 4];
+    uint32_t id[4];
     uint32_t hole;                                           // bit i: keys 16 i .. of the tile have no page
 };
-template <bool ONE>
-__device__ __forceinline__ ManyPages<ONE> many_pages(const KvPages &p, const ManyIds<ONE> &t) {
-    ManyPages<ONE> x;
+__device__ __forceinline__ ManyPages many_pages(const KvPages &p, const int *table, int pages, int key) {
+    ManyPages x;
     x.hole = 0;
 #pragma unroll
-    for (int i = 0; i < (ONE ? 1 : 4); i++) {
-        const bool there = (unsigned)t.id[i] < (unsigned)p.n_pages;
-        if (!there) x.hole |= ONE ? 15u : 1u << i;
-        x.id[i] = there ? (uint32_t)t.id[i] : 0u;
+    for (int i = 0; i < 4; i++) {
+        const int at = (key + 16 * i) >> p.shift, id = at < pages ? table[at] : -1;
+        const bool there = (unsigned)id < (unsigned)p.n_pages;
+        if (!there) x.hole |= 1u << i;
+        x.id[i] = there ? (uint32_t)id : 0u;
     }
     return x;
 }
 // Where the tile's key k (the thread's own) has something that lies `lane`
 // bytes into the page's block for key 0 and `step` bytes further for each key.
-// ONE: a uniform address and the thread's constant offset.
-template <bool ONE>
-__device__ __forceinline__ const unsigned char *many_at(const KvPages &p, const ManyPages<ONE> &pg, int key, uint32_t k,
+__device__ __forceinline__ const unsigned char *many_at(const KvPages &p, const ManyPages &pg, int key, uint32_t k,
                                                         uint32_t lane, uint32_t step) {
     const uint32_t unit = (uint32_t)(p.page_bytes >> 4), rows = 1u << p.shift, at0 = (uint32_t)key & (rows - 1);
-    if (ONE) return p.data + (((uint64_t)pg.id[0] * unit) << 4) + (uint64_t)(at0 * step) + (lane + k * step);
-    const uint32_t id0 = pg.id[0], id1 = pg.id[ONE ? 0 : 1], id2 = pg.id[ONE ? 0 : 2], id3 = pg.id[ONE ? 0 : 3];
+    const uint32_t id0 = pg.id[0], id1 = pg.id[1], id2 = pg.id[2], id3 = pg.id[3];
     const uint32_t a = k & 16 ? id1 : id0, c = k & 16 ? id3 : id2, id = k & 32 ? c : a;
     return p.data + (((uint64_t)id * unit) << 4) + (lane + ((at0 + k) & (rows - 1)) * step);
 }
 
-template <int D, bool Q8, int NT, bool ONE>
-__device__ __forceinline__ void many_load(Stage<D, Q8, NT> &S, const KvPages &p, const ManyPages<ONE> &pg, int kh, int key) {
+template <int D, bool Q8, int NT>
+__device__ __forceinline__ void many_load(Stage<D, Q8, NT> &S, const KvPages &p, const ManyPages &pg, int kh, int key) {
     using T = Stage<D, Q8, NT>;
     const uint32_t tid = threadIdx.x, head = ((uint32_t)kh << p.shift) * (D * T::ES), vo = ((uint32_t)p.hk << p.shift) * (D * T::ES);
 #pragma unroll
     for (int u = 0; u < T::KU; u++) {
         const uint32_t x = u * NT + tid, k = x / T::KROW % MANY_KEYS, c = x % T::KROW;
-        S.k[u] = *(const u32x4 *)many_at<ONE>(p, pg, key, k, head + c * 16, D * T::ES);
+        S.k[u] = *(const u32x4 *)many_at(p, pg, key, k, head + c * 16, D * T::ES);
     }
 #pragma unroll
     for (int u = 0; u < T::VU; u++) {
         const uint32_t x = u * NT + tid, k = x / T::VROW * 4 % MANY_KEYS, c = x % T::VROW;
-        const unsigned char *s = many_at<ONE>(p, pg, key, k, vo + head + c * 4 * T::ES, D * T::ES);
+        const unsigned char *s = many_at(p, pg, key, k, vo + head + c * 4 * T::ES, D * T::ES);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             if (Q8) {
@@ -159,13 +146,13 @@ __device__ __forceinline__ void many_load(Stage<D, Q8, NT> &S, const KvPages &p,
 // The Q8 scales of the tile that S holds: the thread's own, and its share of
 // all of them (every wave over all of the tile's, so that all know the same
 // exponents: lanes 0-31 K's, 32-63 V's).
-template <int D, bool Q8, int NT, bool ONE>
-__device__ __forceinline__ void many_scales(Stage<D, Q8, NT> &S, const KvPages &p, const ManyPages<ONE> &pg, int kh, int key) {
+template <int D, bool Q8, int NT>
+__device__ __forceinline__ void many_scales(Stage<D, Q8, NT> &S, const KvPages &p, const ManyPages &pg, int kh, int key) {
     using T = Stage<D, Q8, NT>;
     if (!Q8) return;
     const uint32_t tid = threadIdx.x, scales = 2 * ((uint32_t)p.hk << p.shift) * D;
     // group g: of K kh G + g, of V behind all of K's
-    auto scale = [&](uint32_t g, uint32_t k) { return many_at<ONE>(p, pg, key, k, scales + (g << p.shift) * 4, 4); };
+    auto scale = [&](uint32_t g, uint32_t k) { return many_at(p, pg, key, k, scales + (g << p.shift) * 4, 4); };
 #pragma unroll
     for (int u = 0; u < T::KU; u++) {
         const uint32_t x = u * NT + tid, k = x / T::KROW % MANY_KEYS, c = x % T::KROW;
@@ -189,14 +176,12 @@ __device__ __forceinline__ void many_scales(Stage<D, Q8, NT> &S, const KvPages &
 
 // Exponents above the tile's K and V scales, of the keys that exist.
 template <int D, bool Q8, int NT>
-__device__ __forceinline__ void many_exps(Stage<D, Q8, NT> &S, uint32_t hole, int key, int len, bool masked, int &ek, int &ev) {
-    if (masked) {
-        const int k = (threadIdx.x & 7) * 8;
+__device__ __forceinline__ void many_exps(Stage<D, Q8, NT> &S, uint32_t hole, int key, int len, int &ek, int &ev) {
+    const int k = (threadIdx.x & 7) * 8;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const bool in = key + k + i < len && !(hole >> (k >> 4) & 1);
-            S.both[i >> 2][i & 3] = in ? finite_or_0(S.both[i >> 2][i & 3]) : 0.0f;
-        }
+    for (int i = 0; i < 8; i++) {
+        const bool in = key + k + i < len && !(hole >> (k >> 4) & 1);
+        S.both[i >> 2][i & 3] = in ? finite_or_0(S.both[i >> 2][i & 3]) : 0.0f;
     }
     float a = fmaxf(S.both[0][0], S.both[0][1]);
 #pragma unroll
@@ -234,15 +219,18 @@ __device__ __forceinline__ int chunk_at(int r, int c) {
     return r * CH + (c ^ (CH >= 16 ? r & 15 : (r / (16 / CH)) & (CH - 1)));
 }
 
-template <int D>
-struct ManyLds {
-    uint16_t k[2][MANY_KEYS * D], v[3][MANY_KEYS * D];       // of tile % 2, % 3
-    uint32_t bad[4][2];                                      // keys of a masked tile whose V is not finite, by tile % 4
+// What the second launch needs of a tile beside its numbers.
+struct ManyHead {
+    int ek, ev;                                              // 2^these > every K and V scale of it
+    uint32_t bad[2];                                         // keys whose V is not finite (it is zeros in the tile)
+    uint32_t hole, unused[3];                                // as ManyPages'
 };
 
+// The tile to k and v, and its keys whose V is not finite to bad (in LDS): a
+// key that some row may not attend must not reach it as 0 * NaN.
 template <int D, bool Q8, int NT>
-__device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, ManyLds<D> &L, uint32_t holes, int kb, int vb, int fb,
-                                           int key, int len, bool masked, int ek, int ev) {
+__device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, uint16_t *kt, uint16_t *vt, uint32_t *bads, uint32_t holes,
+                                           int key, int len, int ek, int ev) {
     using T = Stage<D, Q8, NT>;
     const int tid = threadIdx.x;
 #pragma unroll
@@ -261,10 +249,10 @@ __device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, ManyLds<D> &L, u
                     o[2 * w] = scaled2(0, S.k[u][2 * i + w], 0x0c010c00u, f, c2);
                     o[2 * w + 1] = scaled2(0, S.k[u][2 * i + w], 0x0c030c02u, f, c2);
                 }
-                *(u32x4 *)&L.k[kb][chunk_at<D / 8>(k, 2 * c + i) * 8] = o;
+                *(u32x4 *)&kt[chunk_at<D / 8>(k, 2 * c + i) * 8] = o;
             }
         } else {
-            *(u32x4 *)&L.k[kb][chunk_at<D / 8>(k, c) * 8] = S.k[u];
+            *(u32x4 *)&kt[chunk_at<D / 8>(k, c) * 8] = S.k[u];
         }
     }
 #pragma unroll
@@ -272,7 +260,7 @@ __device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, ManyLds<D> &L, u
         const int x = u * NT + tid;
         if (T::VT % NT && x >= T::VT) break;
         const int k = x / T::VROW * 4, c = x % T::VROW;
-        if (masked) {
+        {
             const bool hole = holes >> (k >> 4) & 1;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -290,7 +278,7 @@ __device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, ManyLds<D> &L, u
 #pragma unroll
                     for (int w = 0; w < T::ES; w++) S.v[u][i][w] = gone || bad ? 0u : S.v[u][i][w];
                 }
-                if (bad && !gone) atomicOr(&L.bad[fb][(k + i) >> 5], 1u << ((k + i) & 31));
+                if (bad && !gone) atomicOr(&bads[(k + i) >> 5], 1u << ((k + i) & 31));
             }
         }
         // the quad's place: 0-3, 8-11, 4-7, 12-15 of each 16 keys
@@ -324,21 +312,64 @@ __device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, ManyLds<D> &L, u
                 o.x = __builtin_amdgcn_perm(S.v[u][1][e >> 1 ? H : 0], S.v[u][0][e >> 1 ? H : 0], sel);
                 o.y = __builtin_amdgcn_perm(S.v[u][3][e >> 1 ? H : 0], S.v[u][2][e >> 1 ? H : 0], sel);
             }
-            *(uint2 *)&L.v[vb][chunk_at<8>(dim, slot >> 3) * 8 + (slot & 7)] = o;
+            *(uint2 *)&vt[chunk_at<8>(dim, slot >> 3) * 8 + (slot & 7)] = o;
         }
     }
 }
 
-template <int D, bool Q8, int NW, bool ONE>
-__global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_many(KvPages p, KvSeqs b, KvRows q, KvRows out, int heads, int group,
-                                                        float scale2, int chunk, int tiles, int vec, KvParts w) {
+#define TILE_THREADS 256
+// Tile blockIdx.x / hk of sequence blockIdx.y, head blockIdx.x % hk: its place
+// in the workspace is (sequence * hk + head) * n + tile.
+template <int D>
+__device__ __forceinline__ unsigned char *tile_at(unsigned char *ws, int hk, int seq, int head, int n, int tile) {
+    return ws + (((long long)seq * hk + head) * n + tile) * (4 * MANY_KEYS * D);
+}
+template <int D, bool Q8>
+__global__ __launch_bounds__(TILE_THREADS) void k_kv_tiles(KvPages p, KvSeqs b, int n, unsigned char *ws, ManyHead *heads) {
+    __shared__ uint32_t bad[2];
+    const int seq = blockIdx.y, kh = blockIdx.x % p.hk, tile = blockIdx.x / p.hk, key = tile * MANY_KEYS;
+    const KvSeq s = kv_seq(b, seq, p.shift);
+    if (key >= s.len || s.n <= 0) return;
+    if (threadIdx.x < 2) bad[threadIdx.x] = 0;
+    __syncthreads();
+    Stage<D, Q8, TILE_THREADS> S;
+    const ManyPages pg = many_pages(p, b.table + seq * b.stride, b.pages, key);
+    many_load<D, Q8, TILE_THREADS>(S, p, pg, kh, key);
+    many_scales<D, Q8, TILE_THREADS>(S, p, pg, kh, key);
+    int ek = 0, ev = 0;
+    if (Q8) many_exps<D, Q8, TILE_THREADS>(S, pg.hole, key, s.len, ek, ev);
+    uint16_t *out = (uint16_t *)tile_at<D>(ws, p.hk, seq, kh, n, tile);
+    many_store<D, Q8, TILE_THREADS>(S, out, out + MANY_KEYS * D, bad, pg.hole, key, s.len, ek, ev);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        ManyHead h = {ek, ev, {bad[0], bad[1]}, pg.hole, {0, 0, 0}};
+        heads[((long long)seq * p.hk + kh) * n + tile] = h;
+    }
+}
+
+typedef const __attribute__((address_space(1))) void *many_gptr;
+typedef __attribute__((address_space(3))) void *many_lptr;
+// All but the last N of the wave's own loads into LDS have arrived, and every
+// wave is here.
+template <int N> __device__ __forceinline__ void many_arrive() {
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+template <int D, bool Q8, int NW>
+__global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_many(KvPages p, KvSeqs b, KvRows q, KvRows out,
+                                                                                  int heads, int group, float scale2,
+                                                                                  int chunk, int tiles, int vec, int per_seq,
+                                                                                  unsigned char *ws, const ManyHead *hd,
+                                                                                  KvParts w) {
     using E = typename std::conditional<Q8, _Float16, __bf16>::type;
     using V8 = typename std::conditional<Q8, f16x8, bf16x8>::type;
-    constexpr int NT = NW * 64, ROWS = NW * 32, KK = D / 16, DT = D / 32;
-    __shared__ __align__(16) ManyLds<D> L;
+    constexpr int ROWS = NW * 32, KK = D / 16, DT = D / 32;
+    constexpr int TILE = MANY_KEYS * D;                      // numbers of K, of V
+    __shared__ __align__(16) uint16_t lk[3 * TILE], lv[4 * TILE];      // of tile % 3, % 4
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
-    const int seq = blockIdx.y, split = blockIdx.x % w.splits, y = blockIdx.x / w.splits;
-    const int kh = y % p.hk, tile = tiles - 1 - y / p.hk;
+    // the sequences of a tile and head next to each other, the tiles with the most keys first
+    const int split = blockIdx.x % w.splits, y = blockIdx.x / w.splits, seq = y % b.n_seq, z = y / b.n_seq;
+    const int kh = z % p.hk, tile = tiles - 1 - z / p.hk;
     const KvSeq s = kv_seq(b, seq, p.shift);
     const int nr = s.n < b.max_rows ? s.n : b.max_rows;
     if ((long long)tile * ROWS >= (long long)nr * group) return;
@@ -352,7 +383,6 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
     int k1 = k0 + chunk;
     const int end = end_of(tile * ROWS + ROWS - 1), all = end_of(tile * ROWS);
     k1 = k1 < end ? k1 : end;
-    const int *table = b.table + seq * b.stride;
 
     const int row = tile * ROWS + wave * 32 + n, j = row / group, head = kh * group + row % group, r = s.r0 + j;
     const bool on = j < nr && (unsigned)r < (unsigned)b.n_rows;
@@ -402,60 +432,47 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
     if (k0 < k1) {
         // Two halves of the block's waves, one of each on every SIMD, take turns:
         // while one has the matrix cores (the values of tile i - 1, the scores of
-        // tile i), the other does tile i's softmax and brings the next tile
-        // into LDS, a barrier between the turns.  With slots of time counted
-        // from 0, half g has the matrix cores for tile i in slot 2 i + g.  Its
-        // share of tile i + 1 + g is stored in the slot after that, so tile j is
-        // stored in slots 2 j - 2 and 2 j - 1: its K is read in slots 2 j and
-        // 2 j + 1, its V in 2 j + 2 and 2 j + 3, and with two buffers for K and
-        // three for V nothing is overwritten before its last reader's slot ends.
-        const int g = wave / (NW / 2), n_tiles = (k1 - k0 + MANY_KEYS - 1) / MANY_KEYS;
-        // of a stored tile, all uniform: the exponents, and its holes | 16 if it is
-        // masked; of tile i, of tile i + 1 (in half 1), of the one just stored
-        int ek0 = 0, ev0 = 0, ek1 = 0, ev1 = 0, ek2 = 0, ev2 = 0;
-        uint32_t how0 = 0, how1 = 0, how2 = 0;
-        if (threadIdx.x < 8) L.bad[threadIdx.x >> 1][threadIdx.x & 1] = 0;
-        // the first turn's values are of a tile that is not: no weights, and numbers to take them times
-        for (int x = threadIdx.x; x < MANY_KEYS * D / 8; x += NT) ((u32x4 *)L.v[2])[x] = u32x4{0, 0, 0, 0};
-        __syncthreads();
-        int eb = -1000;                                      // V's exponent so far
-        auto at = [&](int i) { return k0 + (i < n_tiles ? i : n_tiles - 1) * MANY_KEYS; };
-        Stage<D, Q8, NT> S;
-        ManyPages<ONE> pg;                                        // of the tile in S
-        ManyIds<ONE> next = many_ids<ONE>(p, table, b.pages, at(0));  // of the one behind it
-        auto load = [&](int i) {                             // tile i (the last one again behind the end)
-            pg = many_pages<ONE>(p, next);
-            many_load<D, Q8, NT, ONE>(S, p, pg, kh, at(i));
-            next = many_ids<ONE>(p, table, b.pages, at(i + 1));
+        // tile i), the other does tile i's softmax, a barrier between the turns.
+        // With slots of time counted from 0, half g has the matrix cores for tile
+        // i in slot 2 i + g, reads K of tile i and V of tile i - 1 there, and
+        // starts its share of tile i + 2's loads, which has arrived by the end of
+        // its next turn, slot 2 i + 2 + g.  So tile j's loads run in slots 2 j - 4 to
+        // 2 j - 1, K's readers are in slots 2 j and 2 j + 1, V's in 2 j + 2 and
+        // 2 j + 3: three buffers for K and four for V.
+        const int g = wave / (NW / 2), n_tiles = (k1 - k0 + MANY_KEYS - 1) / MANY_KEYS, t0 = k0 / MANY_KEYS;
+        constexpr int LOADS = TILE * 2 / 1024, PER = 2 * LOADS / NW;         // of 1 KB, of K; a wave's
+        const unsigned char *src = tile_at<D>(ws, p.hk, seq, kh, per_seq, t0) + wave * PER * 1024;
+        // (constant memory to this launch: scalar loads, a tile ahead)
+        typedef const __attribute__((address_space(4))) ManyHead *head_ptr;
+        const head_ptr hds = (head_ptr)(uintptr_t)(hd + (((long long)seq * p.hk + kh) * per_seq + t0));
+        auto head_of = [&](int i) {
+            const head_ptr a = hds + (i < n_tiles ? i : n_tiles - 1);
+            ManyHead x;
+            x.ek = a->ek;
+            x.ev = a->ev;
+            x.bad[0] = a->bad[0];
+            x.bad[1] = a->bad[1];
+            x.hole = a->hole;
+            return x;
         };
-        auto store = [&](int i) {
-            const int key = at(i);
-            const bool masked = key + MANY_KEYS > all || pg.hole;
-            how2 = pg.hole | (masked ? 16u : 0u);
-            if (Q8) {
-                int e;
-                many_exps<D, Q8, NT>(S, pg.hole, key, s.len, masked, ek2, e);
-                eb = eb > e ? eb : e;
-                ev2 = eb;
+        ManyHead head = head_of(0);
+        auto load = [&](int i) {                             // tile i (the last one again behind the end)
+            const unsigned char *a = src + (long long)(i < n_tiles ? i : n_tiles - 1) * (4 * TILE) + lane * 16;
+            char *k = (char *)(lk + i % 3 * TILE), *v = (char *)(lv + (i & 3) * TILE);
+#pragma unroll
+            for (int e = 0; e < PER; e++) {
+                const int x = wave * PER + e;
+                __builtin_amdgcn_global_load_lds((many_gptr)(a + e * 1024),
+                                                 (many_lptr)(x < LOADS ? k + x * 1024 : v + (x - LOADS) * 1024), 16, 0, 0);
             }
-            if (i < n_tiles) many_store<D, Q8, NT>(S, L, pg.hole, i & 1, i % 3, i & 3, key, s.len, masked, ek2, ev2);
         };
         load(0);
-        many_scales<D, Q8, NT, ONE>(S, p, pg, kh, at(0));
-        store(0);
-        ek0 = ek2;
-        ev0 = ev2;
-        how0 = how2;
-        if (g) {
-            load(1);
-            many_scales<D, Q8, NT, ONE>(S, p, pg, kh, at(1));
-            store(1);
-            ek1 = ek2;
-            ev1 = ev2;
-            how1 = how2;
-        }
+        load(1);
+        // the first turn's values are of a tile that is not: no weights, and numbers to take them times
+        for (int x = threadIdx.x; x < TILE / 8; x += NW * 64) ((u32x4 *)(lv + 3 * TILE))[x] = u32x4{0, 0, 0, 0};
         __syncthreads();
-        if (g) __syncthreads();
+        many_arrive<0>();
+        if (g) many_arrive<0>();
         // The fragments of a turn: 4 DT of V for the values of tile i - 1, then 2 KK
         // of K for the scores of tile i, read in fours one four ahead of the
         // instructions that take them.  The scheduling barriers keep it so: left
@@ -466,9 +483,9 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
         const uint32_t lane_v = chunk_at<8>(n, h) * 16, lane_k = chunk_at<D / 8>(n, h) * 16;
         uint32_t row_v = 0, row_k = 0;
         auto fragment = [&](int x) {
-            if (x < NV) return *(const u32x4 *)((const char *)L.v[0] + (row_v ^ (uint32_t)(x / DT << 5)) + x % DT * (32 * 128));
+            if (x < NV) return *(const u32x4 *)((const char *)lv + (row_v ^ (uint32_t)(x / DT << 5)) + x % DT * (32 * 128));
             x -= NV;
-            return *(const u32x4 *)((const char *)L.k[0] + (row_k ^ (uint32_t)(x / 2 << 5)) + x % 2 * (32 * 2 * D));
+            return *(const u32x4 *)((const char *)lk + (row_k ^ (uint32_t)(x / 2 << 5)) + x % 2 * (32 * 2 * D));
         };
         auto product = [&](int x, const u32x4 &f) {
             if (x < NV) {
@@ -482,8 +499,8 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
         auto turn = [&](auto first, auto behind, int i, auto beside) {
             constexpr int A = decltype(first)::value, B = decltype(behind)::value;
             u32x4 f[2][4];
-            row_v = lane_v + (i + 2) % 3 * (uint32_t)sizeof(L.v[0]);
-            row_k = lane_k + (i & 1) * (uint32_t)sizeof(L.k[0]);
+            row_v = lane_v + ((i + 3) & 3) * (2 * TILE);
+            row_k = lane_k + i % 3 * (2 * TILE);
             if (B == NF) {
                 st[0] = f32x16{};
                 st[1] = f32x16{};
@@ -507,33 +524,32 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
         typedef std::integral_constant<int, NF> cf;
         for (int i = 0; i < n_tiles; i++) {
             const int key = k0 + i * MANY_KEYS;
-            turn(c0(), cf(), i, [&]() { load(i + 1 + g); });
-            // (not with the tile's codes: they would take registers through the turn)
-            many_scales<D, Q8, NT, ONE>(S, p, pg, kh, at(i + 1 + g));
-            __syncthreads();
+            turn(c0(), cf(), i, [&]() { load(i + 2); });
+            many_arrive<PER>();
             {
-                if (Q8 && ev0 != ev) {                       // the V scales' unit grew
-                    if (ev != -1000) {
-                        const float f = __builtin_amdgcn_ldexpf(1.0f, ev - ev0);
+                const ManyHead hi = head;
+                head = head_of(i + 1);
+                const bool masked = key + MANY_KEYS > all || hi.hole || hi.bad[0] || hi.bad[1];
+                if (Q8 && hi.ev > ev) {                      // the sums' unit of V's scales grows
+                    const float f = __builtin_amdgcn_ldexpf(1.0f, ev - hi.ev);
 #pragma unroll
-                        for (int d = 0; d < DT; d++) o[d] *= f;
-                    }
-                    ev = ev0;
+                    for (int d = 0; d < DT; d++) o[d] *= f;
+                    ev = hi.ev;
                 }
-                float c = Q8 ? __builtin_amdgcn_ldexpf(cq, ek0) : cq;
+                float c = Q8 ? __builtin_amdgcn_ldexpf(cq, hi.ek) : cq;
                 c = fmaxf(c, 1e-37f);                        // -inf * c stays -inf at a scale of zero
                 float mx = ninf();
-                if (how0 & 16u) {
+                if (masked) {
                     // (the lane's half taken out first, so that what is compared with is constant:
                     // it would be kept in 64 registers through the whole loop)
-                    const uint32_t bad0 = L.bad[i & 3][0] >> (h * 4), bad1 = L.bad[i & 3][1] >> (h * 4);
+                    const uint32_t bad0 = hi.bad[0] >> (h * 4), bad1 = hi.bad[1] >> (h * 4);
                     const int left = lim - key - h * 4;
 #pragma unroll
                     for (int t = 0; t < 2; t++)
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
                             const int k = (e >> 2) * 8 + (e & 3);
-                            const bool in = t * 32 + k < left && !(how0 >> (2 * t + (e >> 3)) & 1);
+                            const bool in = t * 32 + k < left && !(hi.hole >> (2 * t + (e >> 3)) & 1);
                             if (in && ((t ? bad1 : bad0) >> k & 1)) l = __builtin_nanf("");
                             st[t][e] = in ? st[t][e] : ninf();
                         }
@@ -552,7 +568,9 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
                     for (int d = 0; d < DT; d++) o[d] *= f;
                     m = mn;
                 }
-                const float mu = m == ninf() ? 0.0f : m;
+                // weights in the sums' unit: V's tile has its own
+                const float less = Q8 ? (float)(ev - hi.ev) : 0.0f, mu = (m == ninf() ? 0.0f : m) + less;
+                float sum = 0.0f;
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -562,21 +580,13 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
                             const float a = kv_exp2(__builtin_fmaf(st[t][u * 8 + 2 * e], c, -mu));
                             const float d = kv_exp2(__builtin_fmaf(st[t][u * 8 + 2 * e + 1], c, -mu));
                             pw[t][u][e] = pack2<E>(a, d);
-                            l = add2<E>(pw[t][u][e], l);
+                            sum = add2<E>(pw[t][u][e], sum);
                         }
+                l = Q8 ? __builtin_fmaf(sum, kv_exp2(less), l) : l + sum;
             }
-            // the flags of the tile before this one, which nobody reads or sets in this slot
-            if (!g && threadIdx.x < 2) L.bad[(i + 3) & 3][threadIdx.x] = 0;
-            store(i + 1 + g);
-            ek0 = g ? ek1 : ek2;
-            ev0 = g ? ev1 : ev2;
-            how0 = g ? how1 : how2;
-            ek1 = ek2;
-            ev1 = ev2;
-            how1 = how2;
-            __syncthreads();
+            asm volatile("s_barrier" ::: "memory");
         }
-        if (!g) __syncthreads();
+        if (!g) asm volatile("s_barrier" ::: "memory");
         turn(c0(), cv(), n_tiles, []() {});
     }
     l += __shfl_xor(l, 32);
@@ -626,31 +636,58 @@ static bool aligned16(const KvRows &r) {
     return ((uintptr_t)r.p % 16) == 0 && r.row % 8 == 0 && r.head % 8 == 0;
 }
 
+// The tiles of one sequence, and how many sequences' tiles are made at a time:
+// as many as take 1 GiB (the workspace grows no further with the batch).
+static long long seq_tiles(const KvPages &p, const KvSeqs &b) {
+    const long long cap = (long long)b.pages << p.shift, most = b.max_len < cap ? b.max_len : cap;
+    return (most + MANY_KEYS - 1) / MANY_KEYS;
+}
+static int seqs_at_once(const KvPages &p, const KvSeqs &b) {
+    const long long one = seq_tiles(p, b) * p.hk * (4 * MANY_KEYS * p.d), k = one ? (1LL << 30) / one : b.n_seq;
+    return (int)(k < 1 ? 1 : k < b.n_seq ? k : b.n_seq);
+}
+extern "C" long long l98k_kv_many_ws(const KvPages &p, const KvSeqs &b) {
+    return seqs_at_once(p, b) * seq_tiles(p, b) * p.hk * (4LL * MANY_KEYS * p.d + (long long)sizeof(ManyHead));
+}
+
 template <int D, bool Q8>
-static int many(const KvPages &p, const KvSeqs &b, const KvRows &q, const KvRows &o, int heads, float scale2,
-                const KvPlan &x, const KvParts &w, hipStream_t st) {
-    const int vec = aligned16(q) && aligned16(o);
-    const dim3 grid((unsigned)((long long)x.splits * p.hk * x.tiles), b.n_seq);
-#define MANY_LAUNCH(NW, ONE)                                                                                      \
-    hipLaunchKernelGGL((k_kv_many<D, Q8, NW, ONE>), grid, dim3(NW * 64), 0, st, p, b, q, o, heads, heads / p.hk,  \
-                       scale2, x.chunk, x.tiles, vec, w)
-    const bool one = (1 << p.shift) >= MANY_KEYS;
-    if (x.rows == 128) {
-        if (one) MANY_LAUNCH(4, true);
-        else MANY_LAUNCH(4, false);
-    } else {
-        if (one) MANY_LAUNCH(8, true);
-        else MANY_LAUNCH(8, false);
+static int many(const KvPages &p, const KvSeqs &all, const KvRows &q, const KvRows &o, int heads, float scale2,
+                const KvPlan &x, const KvParts &w, unsigned char *ws, hipStream_t st) {
+    const int vec = aligned16(q) && aligned16(o), step = seqs_at_once(p, all);
+    const long long n = seq_tiles(p, all), blocks = (long long)x.splits * p.hk * x.tiles * step;
+    if (n * p.hk > INT_MAX || blocks > INT_MAX) return -1;
+    ManyHead *hd = (ManyHead *)(ws + step * n * p.hk * (4LL * MANY_KEYS * D));
+    for (int i = 0; i < all.n_seq; i += step) {
+        KvSeqs b = all;
+        b.table += i * b.stride;
+        b.kv_len += i;
+        b.row0 += i;
+        b.n_seq = all.n_seq - i < step ? all.n_seq - i : step;
+        if (n) {
+            hipLaunchKernelGGL((k_kv_tiles<D, Q8>), dim3((unsigned)(n * p.hk), b.n_seq), dim3(TILE_THREADS), 0, st, p, b,
+                               (int)n, ws, hd);
+            const int rc = (int)hipGetLastError();
+            if (rc) return rc;
+        }
+        const dim3 grid((unsigned)((long long)x.splits * p.hk * x.tiles * b.n_seq));
+        if (x.rows == 128)
+            hipLaunchKernelGGL((k_kv_many<D, Q8, 4>), grid, dim3(256), 0, st, p, b, q, o, heads, heads / p.hk, scale2,
+                               x.chunk, x.tiles, vec, (int)n, ws, hd, w);
+        else
+            hipLaunchKernelGGL((k_kv_many<D, Q8, 8>), grid, dim3(512), 0, st, p, b, q, o, heads, heads / p.hk, scale2,
+                               x.chunk, x.tiles, vec, (int)n, ws, hd, w);
+        const int rc = (int)hipGetLastError();
+        if (rc) return rc;
     }
-    return (int)hipGetLastError();
+    return 0;
 }
 
 extern "C" int l98k_kv_many(const KvPages &p, int q8, const KvSeqs &b, const KvRows &q, const KvRows &o, int heads,
-                            float scale2, const KvPlan &x, const KvParts &w, hipStream_t st) {
-#define MANY_D(DD)                                                                  \
-    if (p.d == DD)                                                                  \
-        return q8 ? many<DD, true>(p, b, q, o, heads, scale2, x, w, st)             \
-                  : many<DD, false>(p, b, q, o, heads, scale2, x, w, st)
+                            float scale2, const KvPlan &x, const KvParts &w, void *ws, hipStream_t st) {
+#define MANY_D(DD)                                                                                         \
+    if (p.d == DD)                                                                                         \
+        return q8 ? many<DD, true>(p, b, q, o, heads, scale2, x, w, (unsigned char *)ws, st)               \
+                  : many<DD, false>(p, b, q, o, heads, scale2, x, w, (unsigned char *)ws, st)
     MANY_D(32);
     MANY_D(64);
     MANY_D(128);

@@ -68,5 +68,7 @@ struct KvPlan {
 };
 
 extern "C" int l98k_kv_many(const KvPages &p, int q8, const KvSeqs &b, const KvRows &q, const KvRows &o, int heads,
-                            float scale2, const KvPlan &x, const KvParts &w, hipStream_t st);
+                            float scale2, const KvPlan &x, const KvParts &w, void *ws, hipStream_t st);
+// bytes of its workspace, a multiple of 16
+extern "C" long long l98k_kv_many_ws(const KvPages &p, const KvSeqs &b);
 #endif
