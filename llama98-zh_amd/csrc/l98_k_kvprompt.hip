@@ -439,7 +439,8 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
         // its next turn, slot 2 i + 2 + g.  So tile j's loads run in slots 2 j - 4 to
         // 2 j - 1, K's readers are in slots 2 j and 2 j + 1, V's in 2 j + 2 and
         // 2 j + 3: three buffers for K and four for V.
-        const int g = wave / (NW / 2), n_tiles = (k1 - k0 + MANY_KEYS - 1) / MANY_KEYS, t0 = k0 / MANY_KEYS;
+        // (Four waves, of small calls, have a SIMD each: they are all half 0.)
+        const int g = NW == 8 ? wave / 4 : 0, n_tiles = (k1 - k0 + MANY_KEYS - 1) / MANY_KEYS, t0 = k0 / MANY_KEYS;
         constexpr int LOADS = TILE * 2 / 1024, PER = 2 * LOADS / NW;         // of 1 KB, of K; a wave's
         const unsigned char *src = tile_at<D>(ws, p.hk, seq, kh, per_seq, t0) + wave * PER * 1024;
         // (constant memory to this launch: scalar loads, a tile ahead)
@@ -495,18 +496,25 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
                 st[x % 2] = mfma32(as<V8>(f), qf[x / 2], st[x % 2]);
             }
         };
-        // `beside` is done while the matrix cores have the first four
+        // The first four, of V, are read before the turn's barrier (their tile is
+        // there for two turns already); `beside` is done while the matrix cores
+        // have them.
+        u32x4 f0[4] = {};
+        auto first_four = [&](int i) {                       // of turn i
+            row_v = lane_v + ((i + 3) & 3) * (2 * TILE);
+#pragma unroll
+            for (int e = 0; e < 4; e++) f0[e] = fragment(e);
+        };
         auto turn = [&](auto first, auto behind, int i, auto beside) {
             constexpr int A = decltype(first)::value, B = decltype(behind)::value;
             u32x4 f[2][4];
-            row_v = lane_v + ((i + 3) & 3) * (2 * TILE);
             row_k = lane_k + i % 3 * (2 * TILE);
             if (B == NF) {
                 st[0] = f32x16{};
                 st[1] = f32x16{};
             }
 #pragma unroll
-            for (int e = 0; e < 4; e++) f[0][e] = fragment(A + e);
+            for (int e = 0; e < 4; e++) f[0][e] = f0[e];
 #pragma unroll
             for (int x = A; x < B; x += 4) {
                 if (x + 4 < B)
@@ -522,6 +530,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
         typedef std::integral_constant<int, 0> c0;
         typedef std::integral_constant<int, NV> cv;
         typedef std::integral_constant<int, NF> cf;
+        first_four(0);
         for (int i = 0; i < n_tiles; i++) {
             const int key = k0 + i * MANY_KEYS;
             turn(c0(), cf(), i, [&]() { load(i + 2); });
@@ -584,6 +593,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
                         }
                 l = Q8 ? __builtin_fmaf(sum, kv_exp2(less), l) : l + sum;
             }
+            first_four(i + 1);
             asm volatile("s_barrier" ::: "memory");
         }
         if (!g) asm volatile("s_barrier" ::: "memory");
