@@ -614,7 +614,7 @@ class Engine:
 # ------------------------------------------------ paged key-value cache ---
 
 KV_FORMATS = {"q8": 0, "bf16": 1}
-_KV_TYPES = {"torch.float32": 0, "torch.bfloat16": 1}
+_kv_types = {}                  # torch dtype -> L98_F32 / L98_BF16 (torch is loaded by the first call's tensors)
 
 
 def _kv_stream(stream, like):
@@ -622,14 +622,18 @@ def _kv_stream(stream, like):
     or the current stream of the tensor's device."""
     if stream is None:
         import torch
-        return torch.cuda.current_stream(like.device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(like.get_device())
     return getattr(stream, "cuda_stream", stream)
 
 
 def _kv_type(t, name):
-    code = _KV_TYPES.get(str(t.dtype))
+    code = _kv_types.get(t.dtype)
     if code is None:
-        raise ValueError(f"{name} is {t.dtype}: float32 and bfloat16 are taken")
+        import torch
+        _kv_types.update({torch.float32: 0, torch.bfloat16: 1})
+        code = _kv_types.get(t.dtype)
+        if code is None:
+            raise ValueError(f"{name} is {t.dtype}: float32 and bfloat16 are taken")
     return code
 
 
@@ -637,12 +641,13 @@ def _kv_rows(t, name, n_rows, heads, dim):
     """L98KvRows of a [rows, heads, dim] tensor on the GPU."""
     if not t.is_cuda:
         raise ValueError(f"{name} is not on a GPU")
-    if t.dim() != 3 or t.shape[0] < n_rows or (heads and t.shape[1] != heads) or t.shape[2] != dim:
-        raise ValueError(f"{name} has the shape {tuple(t.shape)}: "
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[0] < n_rows or (heads and shape[1] != heads) or shape[2] != dim:
+        raise ValueError(f"{name} has the shape {tuple(shape)}: "
                          f"[{n_rows} or more, {heads or 'heads'}, {dim}] is taken")
-    if t.stride(2) != 1:
-        raise ValueError(f"{name}'s last dimension has the stride {t.stride(2)}: 1 is taken")
-    return L98KvRows(t.data_ptr(), t.stride(0), t.stride(1))
+    if stride[2] != 1:
+        raise ValueError(f"{name}'s last dimension has the stride {stride[2]}: 1 is taken")
+    return L98KvRows(t.data_ptr(), stride[0], stride[1])
 
 
 class KvBatch:
@@ -740,7 +745,7 @@ class KvPool:
         err = C.create_string_buffer(256)
         self._done(self.lib.l98_kv_attend(
             self.c, layer, batch.c, rq, ro, q.shape[1], code, scale, ws.data_ptr() if ws is not None else None,
-            ws.numel() * ws.element_size() if ws is not None else 0, _kv_stream(stream, q), err, 256), err)
+            ws.nbytes if ws is not None else 0, _kv_stream(stream, q), err, 256), err)
         return out
 
     def copy_pages(self, src, dst, stream=None):

@@ -214,7 +214,8 @@ __global__ __launch_bounds__(KV_THREADS) void k_kv_read(KvPages p, KvSeqs b, KvR
 // Whole pages, 16 bytes a lane and load, KV_COPY_UNROLL loads in flight (the
 // index clamped instead of a branch around each load).
 #define KV_COPY_UNROLL 4
-__global__ __launch_bounds__(KV_THREADS) void k_kv_copy(unsigned char *data, long long page_bytes, KvMoves m) {
+template <int N>
+__global__ __launch_bounds__(KV_THREADS) void k_kv_copy(unsigned char *data, long long page_bytes, KvMoves<N> m) {
     typedef uint32_t v4 __attribute__((ext_vector_type(4)));
     const v4 *s = (const v4 *)(data + m.src[blockIdx.y] * page_bytes);
     v4 *d = (v4 *)(data + m.dst[blockIdx.y] * page_bytes);
@@ -266,16 +267,22 @@ extern "C" int l98k_kv_read(const KvPages &p, int q8, const KvSeqs &b, const KvR
     KV_ROWS_DISPATCH(k_kv_read);
 }
 
+template <int N>
+static int copy_some(unsigned char *data, long long page_bytes, const int *src, const int *dst, int n, hipStream_t st) {
+    const long long per = (long long)KV_THREADS * KV_COPY_UNROLL * 16;
+    KvMoves<N> m = {};
+    for (int u = 0; u < n; u++) { m.src[u] = src[u]; m.dst[u] = dst[u]; }
+    hipLaunchKernelGGL((k_kv_copy<N>), dim3((unsigned)((page_bytes + per - 1) / per), n), dim3(KV_THREADS), 0, st, data,
+                       page_bytes, m);
+    return (int)hipGetLastError();
+}
+// A launch's arguments hold at most 4 KB; a fork's few copies take a launch of
+// few arguments.
 extern "C" int l98k_kv_copy(unsigned char *data, long long page_bytes, const int *src, const int *dst, int n,
                             hipStream_t st) {
-    const long long per = (long long)KV_THREADS * KV_COPY_UNROLL * 16;
-    for (int i = 0; i < n; i += KV_COPY_MAX) {
-        const int k = n - i < KV_COPY_MAX ? n - i : KV_COPY_MAX;
-        KvMoves m = {};
-        for (int u = 0; u < k; u++) { m.src[u] = src[i + u]; m.dst[u] = dst[i + u]; }
-        hipLaunchKernelGGL(k_kv_copy, dim3((unsigned)((page_bytes + per - 1) / per), k), dim3(KV_THREADS), 0, st, data,
-                           page_bytes, m);
-        const int rc = (int)hipGetLastError();
+    if (n <= 16) return copy_some<16>(data, page_bytes, src, dst, n, st);
+    for (int i = 0; i < n; i += 448) {
+        const int rc = copy_some<448>(data, page_bytes, src + i, dst + i, n - i < 448 ? n - i : 448, st);
         if (rc) return rc;
     }
     return 0;

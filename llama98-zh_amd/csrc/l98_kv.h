@@ -28,9 +28,10 @@ struct KvRows {
     long long row, head;
 };
 
-#define KV_COPY_MAX 448           // page pairs that one launch's arguments hold
+// page pairs of one launch, in its arguments
+template <int N>
 struct KvMoves {
-    int src[KV_COPY_MAX], dst[KV_COPY_MAX];
+    int src[N], dst[N];
 };
 
 // One sequence of a batch as a kernel sees it: its first row, its number of
