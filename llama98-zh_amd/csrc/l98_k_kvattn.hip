@@ -253,13 +253,13 @@ __device__ __forceinline__ void few_scores(const FewAcc<D, Q8, BF, MT> &A, const
 // have a page; masked: some row may not attend some of the keys, or they are
 // not all there.
 template <int D, bool Q8, bool BF, int MT>
-__device__ __forceinline__ void few_values(FewAcc<D, Q8, BF, MT> &A, FewTile<D, Q8, BF> &T, const float *sc,
+__device__ __forceinline__ void few_values(FewAcc<D, Q8, BF, MT> &A, FewTile<D, Q8, BF> &T, float *sc,
                                            f32x4 (&s)[MT][2], int key, int len, bool there0, bool there1, bool masked,
                                            float vex) {
     using F = Few<D, Q8, BF>;
     using E = typename F::E;
     using V8 = typename F::V8;
-    const int h = (threadIdx.x & 63) >> 4;
+    const int lane = threadIdx.x & 63, h = lane >> 4;
     // Q8 weights are p * (V's scale): 2^ex > every scale that the row attends
     // of the tile (vex: all of them), and s + ex bounds their logarithm.  They
     // may reach 2^15; a raise of the running maximum brings them to 2^11.
@@ -278,9 +278,28 @@ __device__ __forceinline__ void few_values(FewAcc<D, Q8, BF, MT> &A, FewTile<D, 
                 s[m][i >> 2][i & 3] = in ? s[m][i >> 2][i & 3] : ninf();
                 if (Q8)
 #pragma unroll
-                    for (int g = 0; g < F::NG; g++) vx = fmaxf(vx, in ? sc[(F::NG + g) * FEW_KEYS + k] : 0.0f);
+                    for (int g = 0; g < F::NG; g++) {
+                        const float v = sc[(F::NG + g) * FEW_KEYS + k];
+                        const bool bad = (u_from_f(v) & 0x7F800000u) == 0x7F800000u;
+                        if (in && bad) A.l[m] = __builtin_nanf("");
+                        vx = fmaxf(vx, in && !bad ? v : 0.0f);
+                    }
             }
             cand[m] = Q8 ? (float)((int)(u_from_f(vx) >> 23) - 126) : 0.0f;
+        }
+        if (Q8) {
+            // A scale that is not finite becomes zero, so that it does not reach the
+            // rows that may not attend its key as 0 * NaN; those that attend it have
+            // NaN by their sum.
+            if (lane < 2 * F::NG * 8 && lane >= F::NG * 8) {
+                f32x4 v = *(f32x4 *)(sc + lane * 4);
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[i] = (u_from_f(v[i]) & 0x7F800000u) == 0x7F800000u ? 0.0f : v[i];
+                *(f32x4 *)(sc + lane * 4) = v;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
     } else {
 #pragma unroll
@@ -345,12 +364,6 @@ __device__ __forceinline__ void few_values(FewAcc<D, Q8, BF, MT> &A, FewTile<D, 
                 if (Q8) {
                     a *= vs[t][e];
                     b *= vs[t][e + 1];
-                    if (masked) {                            // 0 * a scale that is not finite
-                        const bool there = t ? there1 : there0;
-                        const int k = key + t * 16 + h * 4 + e;
-                        a = there && k < A.lim[m] ? a : 0.0f;
-                        b = there && k + 1 < A.lim[m] ? b : 0.0f;
-                    }
                 }
                 uint32_t x[F::NP];
                 parts2<E, F::NP>(a, b, x);
