@@ -9,6 +9,9 @@
 #include "l98_kv.h"
 
 #define KV_THREADS 256
+// Four units a lane where one each would be more blocks than the chip holds at
+// once, 8 on each of 256 CUs.
+#define KV_ALL 2048
 
 template <class T> __device__ __forceinline__ float kv_f32(T x) { return (float)x; }
 
@@ -48,54 +51,67 @@ __device__ __forceinline__ void kv_store(T *x, bool vec, const float *v) {
     }
 }
 
-// A row of one head of K or V belongs to 16 lanes, E = D / 16 elements each:
-// of K (and of a bf16 row) the lane's own consecutive dimensions, of a Q8 V
-// row the dimensions t * 16 + lane, so that either way a lane's E codes lie
-// together in the page.
-struct KvUnit {
-    int lane, which, head, row;          // which: 0 K, 1 V; row: of the arrays, -1 for none
-    const unsigned char *page;           // null: the position has no page
+// A piece, the row of one head of K or V, belongs to 16 lanes, E = D / 16
+// consecutive dimensions each.  A Q8 piece's codes are made that way too, and
+// V's then change lanes through LDS: in the page lane n's E codes are the
+// dimensions t * 16 + n.  A block's 16 groups of lanes take 16 rows, or with
+// fewer rows several pieces of each, and U pieces one after the other whose
+// loads are in flight together: a page has a head's rows side by side and of
+// their scales a group's, and what a row needs (its page, its places) is found
+// once.  (Appending 19,000 bf16 rows of 4 heads of 128, 61 MB: 17 us and reading
+// them 13, where a large copy would take 12.  With each piece on its own 24 and
+// 16: that is bound by the instructions that find its places.  With V read from
+// the caller's rows in the page's order, two bytes a load, appending took 32.)
+struct KvRow {
+    int row;                             // of the arrays, -1 for none
+    unsigned char *page;                 // null: the position has no page
     int off;                             // its row in the page
+    int w0, step;                        // its first piece, and from one to the next; K's heads come before V's
 };
-__device__ __forceinline__ KvUnit kv_unit(const KvPages &p, const KvSeqs &b) {
-    KvUnit u;
-    u.lane = threadIdx.x & 15;
+// lr: log2 of a block's rows; parts: blocks of a row
+__device__ __forceinline__ KvRow kv_row(const KvPages &p, const KvSeqs &b, int lr, unsigned parts, int U) {
+    KvRow u;
     const KvSeq s = kv_seq(b, blockIdx.y, p.shift);
-    const long long i = (long long)blockIdx.x * (KV_THREADS / 16) + (threadIdx.x >> 4);
-    const int per = 2 * p.hk;
-    const int j = (int)(i / per), w = (int)(i % per);
-    u.which = w & 1;
-    u.head = w >> 1;
-    const int r = s.r0 + j, pos = s.pos0 + j;
+    const unsigned group = blockIdx.x / parts, slot = threadIdx.x >> 4;
+    const long long j = ((long long)group << lr) + (slot & ((1u << lr) - 1));
+    u.step = KV_THREADS / 16 >> lr;
+    u.w0 = (int)(blockIdx.x - group * parts) * U * u.step + (int)(slot >> lr);
+    const int r = s.r0 + (int)j, pos = s.pos0 + (int)j;
     u.row = j < s.n && j < b.max_rows && (unsigned)r < (unsigned)b.n_rows ? r : -1;
     u.page = nullptr;
     u.off = 0;
     if (u.row >= 0 && pos >= 0 && pos < s.len) {
         const int id = b.table[blockIdx.y * b.stride + (pos >> p.shift)];
-        if ((unsigned)id < (unsigned)p.n_pages) u.page = kv_page(p, id);
+        if ((unsigned)id < (unsigned)p.n_pages) u.page = const_cast<unsigned char *>(kv_page(p, id));
         u.off = pos & ((1 << p.shift) - 1);
     }
     return u;
 }
-// offsets in a page's block: a row's numbers (es bytes each), and its scale of group g
+// offsets in a page's block: piece w's numbers (es bytes each), and its scale of group g
 template <int D>
-__device__ __forceinline__ long long kv_at(const KvPages &p, const KvUnit &u, int es) {
-    return ((((long long)u.which * p.hk + u.head) << p.shift) + u.off) * D * es;
+__device__ __forceinline__ long long kv_at(const KvPages &p, int off, int w, int es) {
+    return (((long long)w << p.shift) + off) * D * es;
 }
 template <int D>
-__device__ __forceinline__ long long kv_scale_at(const KvPages &p, const KvUnit &u, int g) {
-    return (((long long)2 * p.hk << p.shift) * D) +
-           ((((((long long)u.which * p.hk + u.head) * (D / 32)) + g) << p.shift) + u.off) * 4;
+__device__ __forceinline__ long long kv_scale_at(const KvPages &p, int off, int w, int g) {
+    return (((long long)2 * p.hk << p.shift) * D) + ((((long long)w * (D / 32) + g) << p.shift) + off) * 4;
+}
+// where piece w of a row lies in the caller's arrays
+template <class T>
+__device__ __forceinline__ T *kv_place(const KvPages &p, const KvRows &k, const KvRows &v, int row, int w) {
+    const bool second = w >= p.hk;
+    return (T *)(second ? v.p : k.p) + (row * (second ? v.row : k.row) + (w - (second ? p.hk : 0)) * (second ? v.head : k.head));
 }
 
-// q8_scale_inv with the factor 127 * (1 / max) instead of 127 / max: what a
-// torch program that fills pages itself gets from 127.0 / max.  (Some of the
-// factors differ in the last bit, and with them about one code in a million
-// by one.)
+// Scale and factor of a Q8 group: scale max * (1 / 127), factor 127 * (1 / max)
+// (what a torch program that fills pages itself gets from 127.0 / max: against
+// 127 / max some factors differ in the last bit, and with them about one code
+// in a million by one).  A group of zeros, with NaN or too small: 1 and 0.
 __device__ __forceinline__ void kv_scale_inv(float amax, float *sg, float *inv) {
-    float unused;
-    q8_scale_inv(amax, sg, &unused);
-    *inv = unused == 0.0f ? 0.0f : 127.0f * (1.0f / amax);
+    const float s = amax * (1.0f / 127.0f);
+    const bool live = amax > 0.0f && !(s < 1.0e-30f);
+    *sg = live ? s : 1.0f;
+    *inv = live ? 127.0f * (1.0f / amax) : 0.0f;
 }
 
 __device__ __forceinline__ uint32_t max_over(uint32_t v, int lanes) {    // over aligned groups of `lanes`
@@ -106,108 +122,139 @@ __device__ __forceinline__ uint32_t max_over(uint32_t v, int lanes) {    // over
     return v;
 }
 
-template <class T, int D, bool Q8>
-__global__ __launch_bounds__(KV_THREADS) void k_kv_append(KvPages p, KvSeqs b, KvRows k, KvRows v, int vec) {
-    constexpr int E = D / 16;
-    const KvUnit u = kv_unit(p, b);
-    const KvRows &src = u.which ? v : k;
-    float x[E];
+// E codes of a lane as they lie together, in the low bytes
+template <int E> struct KvCodes {
+    uint32_t w[(E + 3) / 4];
+    __device__ __forceinline__ void load(const unsigned char *s) {
+        if (E == 8) {
+            const uint2 t = *(const uint2 *)s;
+            w[0] = t.x;
+            w[E == 8 ? 1 : 0] = t.y;
+        } else if (E == 4) {
+            w[0] = *(const uint32_t *)s;
+        } else {
+            w[0] = *(const uint16_t *)s;
+        }
+    }
+    __device__ __forceinline__ void store(unsigned char *s) const {
+        if (E == 8) *(uint2 *)s = make_uint2(w[0], w[E == 8 ? 1 : 0]);
+        else if (E == 4) *(uint32_t *)s = w[0];
+        else *(uint16_t *)s = (uint16_t)w[0];
+    }
+    __device__ __forceinline__ uint32_t operator[](int i) const { return (w[i / 4] >> (8 * (i & 3))) & 255u; }
+};
+// The lanes of a row are of one wave: what one of them wrote to LDS is there
+// for the others behind this.
+__device__ __forceinline__ void kv_lanes() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+// K's dimension c*32 + h*8 + j lies at byte h*(D/4) + c*8 + j
+template <int D> __device__ __forceinline__ int kv_k_byte(int d) { return ((d & 31) >> 3) * (D / 4) + (d >> 5) * 8 + (d & 7); }
+
+template <class T, int D, bool Q8, int U>
+__global__ __launch_bounds__(KV_THREADS) void k_kv_append(KvPages p, KvSeqs b, KvRows k, KvRows v, int vec, int lr, unsigned parts) {
+    constexpr int E = D / 16, N = KV_THREADS / 16;
+    __shared__ __align__(16) unsigned char rows[Q8 ? U : 1][Q8 ? N : 1][D];
+    const KvRow u = kv_row(p, b, lr, parts, U);
+    const int lane = threadIdx.x & 15, slot = threadIdx.x >> 4, d0 = lane * E;
+    float x[U][E];
+    // the shuffles below take every lane of the wave; one without a piece reads a row's first
 #pragma unroll
-    for (int i = 0; i < E; i++) x[i] = 0.0f;
-    const bool live = u.page != nullptr;
-    const T *s = (const T *)src.p + (live ? u.row * src.row + u.head * src.head : 0);
+    for (int i = 0; i < U; i++) {
+        const int w = u.w0 + i * u.step;
+        kv_load<T, E>(kv_place<const T>(p, k, v, u.page ? u.row : 0, w < 2 * p.hk ? w : 0) + d0, vec, x[i]);
+    }
     if (!Q8) {
-        if (!live) return;
-        kv_load<T, E>(s + u.lane * E, vec, x);
-        kv_store<__bf16, E>((__bf16 *)(u.page + kv_at<D>(p, u, 2)) + u.lane * E, true, x);
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int w = u.w0 + i * u.step;
+            if (u.page && w < 2 * p.hk) kv_store<__bf16, E>((__bf16 *)(u.page + kv_at<D>(p, u.off, w, 2)) + d0, true, x[i]);
+        }
         return;
     }
-    // the shuffles below take every lane of the wave
-    if (live) {
-        if (u.which == 0) {
-            kv_load<T, E>(s + u.lane * E, vec, x);
-        } else {
+    KvCodes<E> c[U];
+    float sg[U];
 #pragma unroll
-            for (int t = 0; t < E; t++) x[t] = (float)s[t * 16 + u.lane];
+    for (int i = 0; i < U; i++) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const uint32_t a = u_from_f(x[i][e]) & 0x7FFFFFFFu;
+            m = a > m ? a : m;
         }
-    }
-    uint32_t c[(E + 3) / 4] = {};
-    float sg, inv;
-    uint32_t am[E / 2];
-#pragma unroll
-    for (int g = 0; g < E / 2; g++) {
-        const uint32_t a = u_from_f(x[2 * g]) & 0x7FFFFFFFu, e = u_from_f(x[2 * g + 1]) & 0x7FFFFFFFu;
-        am[g] = a > e ? a : e;
-    }
-    if (u.which == 0) {
-        uint32_t m = am[0];
-#pragma unroll
-        for (int g = 1; g < E / 2; g++) m = am[g] > m ? am[g] : m;
         m = max_over(m, 32 / E);
+        float inv;
+        kv_scale_inv(f_from_u(m), &sg[i], &inv);
+        c[i] = KvCodes<E>();
+        // x + 1.5 * 2^23 has x rounded half to even in its lowest byte, 128 more
+        // is the sign bit turned.  |x * inv| < 127.5 where the factor is not 0;
+        // where it is, all codes are 0 whatever x holds.
 #pragma unroll
-        for (int g = 0; g < E / 2; g++) am[g] = m;
-    } else {
+        for (int e = 0; e < E; e++) c[i].w[e / 4] |= (u_from_f(x[i][e] * inv + 12582912.0f) & 255u) << (8 * (e & 3));
 #pragma unroll
-        for (int g = 0; g < E / 2; g++) am[g] = max_over(am[g], 16);
+        for (int e = 0; e < (E + 3) / 4; e++) c[i].w[e] = (inv == 0.0f ? 0u : c[i].w[e]) ^ 0x80808080u;
+        c[i].store(rows[i][slot] + d0);
     }
+    kv_lanes();
 #pragma unroll
-    for (int g = 0; g < E / 2; g++) {
-        kv_scale_inv(f_from_u(am[g]), &sg, &inv);
-        if (live && (u.which == 0 ? g == 0 && u.lane % (32 / E) == 0 : u.lane == 0))
-            *(float *)(u.page + kv_scale_at<D>(p, u, u.which == 0 ? u.lane * E / 32 : g)) = sg;
+    for (int i = 0; i < U; i++) {
+        const int w = u.w0 + i * u.step;
+        if (w >= p.hk) {
 #pragma unroll
-        for (int i = 2 * g; i < 2 * g + 2; i++) {
-            int qi = d_q8_round(x[i] * inv);
-            qi = qi > 127 ? 127 : qi;
-            qi = qi < -127 ? -127 : qi;
-            c[i / 4] |= (uint32_t)(qi + 128) << (8 * (i & 3));
+            for (int e = 0; e < (E + 3) / 4; e++) c[i].w[e] = 0;
+#pragma unroll
+            for (int t = 0; t < E; t++) c[i].w[t / 4] |= (uint32_t)rows[i][slot][t * 16 + lane] << (8 * (t & 3));
         }
+        if (!u.page || w >= 2 * p.hk) continue;
+        if (lane % (32 / E) == 0) *(float *)(u.page + kv_scale_at<D>(p, u.off, w, d0 / 32)) = sg[i];
+        c[i].store(u.page + kv_at<D>(p, u.off, w, 1) + (w >= p.hk ? d0 : kv_k_byte<D>(d0)));
     }
-    if (!live) return;
-    // K: dimension c*32 + h*8 + j lies at byte h*(D/4) + c*8 + j
-    const int d0 = u.lane * E;
-    const int at = u.which ? d0 : ((d0 & 31) >> 3) * (D / 4) + (d0 >> 5) * 8 + (d0 & 7);
-    unsigned char *o = const_cast<unsigned char *>(u.page) + kv_at<D>(p, u, 1) + at;
-    if (E == 8) *(uint2 *)o = make_uint2(c[0], c[E == 8 ? 1 : 0]);
-    else if (E == 4) *(uint32_t *)o = c[0];
-    else *(uint16_t *)o = (uint16_t)c[0];
 }
 
-template <class T, int D, bool Q8>
-__global__ __launch_bounds__(KV_THREADS) void k_kv_read(KvPages p, KvSeqs b, KvRows k, KvRows v, int vec) {
-    constexpr int E = D / 16;
-    const KvUnit u = kv_unit(p, b);
-    if (u.row < 0) return;
-    const KvRows &dst = u.which ? v : k;
-    T *o = (T *)dst.p + (u.row * dst.row + u.head * dst.head);
-    float x[E];
-#pragma unroll
-    for (int i = 0; i < E; i++) x[i] = 0.0f;
+template <class T, int D, bool Q8, int U>
+__global__ __launch_bounds__(KV_THREADS) void k_kv_read(KvPages p, KvSeqs b, KvRows k, KvRows v, int vec, int lr, unsigned parts) {
+    constexpr int E = D / 16, N = KV_THREADS / 16;
+    __shared__ __align__(16) unsigned char rows[Q8 ? U : 1][Q8 ? N : 1][D];
+    const KvRow u = kv_row(p, b, lr, parts, U);
+    const int lane = threadIdx.x & 15, slot = threadIdx.x >> 4, d0 = lane * E;
+    float x[U][E];
     if (!Q8) {
-        if (u.page) kv_load<__bf16, E>((const __bf16 *)(u.page + kv_at<D>(p, u, 2)) + u.lane * E, true, x);
-        kv_store<T, E>(o + u.lane * E, vec, x);
-        return;
-    }
-    if (u.page) {
-        const int d0 = u.lane * E;
-        const int at = u.which ? d0 : ((d0 & 31) >> 3) * (D / 4) + (d0 >> 5) * 8 + (d0 & 7);
-        const unsigned char *c = u.page + kv_at<D>(p, u, 1) + at;
-        uint32_t w[(E + 3) / 4];
-        if (E == 8) { const uint2 t = *(const uint2 *)c; w[0] = t.x; w[E == 8 ? 1 : 0] = t.y; }
-        else if (E == 4) w[0] = *(const uint32_t *)c;
-        else w[0] = *(const uint16_t *)c;
 #pragma unroll
-        for (int i = 0; i < E; i++) {
-            const int g = u.which ? i / 2 : d0 / 32;
-            const float sg = *(const float *)(u.page + kv_scale_at<D>(p, u, g));
-            x[i] = (float)((int)((w[i / 4] >> (8 * (i & 3))) & 255u) - 128) * sg;
+        for (int i = 0; i < U; i++) {
+            const int w = u.w0 + i * u.step;
+#pragma unroll
+            for (int e = 0; e < E; e++) x[i][e] = 0.0f;
+            if (u.page && w < 2 * p.hk) kv_load<__bf16, E>((const __bf16 *)(u.page + kv_at<D>(p, u.off, w, 2)) + d0, true, x[i]);
+        }
+    } else {
+        KvCodes<E> c[U];
+        float sg[U];
+        const unsigned char *page = u.page ? u.page : p.data;      // (without one: a row of page 0, not used)
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int w = u.w0 + i * u.step, a = w < 2 * p.hk ? w : 0;
+            c[i].load(page + kv_at<D>(p, u.off, a, 1) + (a >= p.hk ? d0 : kv_k_byte<D>(d0)));
+            sg[i] = *(const float *)(page + kv_scale_at<D>(p, u.off, a, d0 / 32));
+        }
+#pragma unroll
+        for (int i = 0; i < U; i++)
+            if (u.w0 + i * u.step >= p.hk)
+#pragma unroll
+                for (int t = 0; t < E; t++) rows[i][slot][t * 16 + lane] = (unsigned char)c[i][t];
+        kv_lanes();
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            if (u.w0 + i * u.step >= p.hk) c[i].load(rows[i][slot] + d0);
+#pragma unroll
+            for (int e = 0; e < E; e++) x[i][e] = u.page ? (float)((int)c[i][e] - 128) * sg[i] : 0.0f;
         }
     }
-    if (u.which == 0) {
-        kv_store<T, E>(o + u.lane * E, vec, x);
-    } else {
 #pragma unroll
-        for (int t = 0; t < E; t++) o[t * 16 + u.lane] = (T)x[t];
+    for (int i = 0; i < U; i++) {
+        const int w = u.w0 + i * u.step;
+        if (u.row >= 0 && w < 2 * p.hk) kv_store<T, E>(kv_place<T>(p, k, v, u.row, w) + d0, vec, x[i]);
     }
 }
 
@@ -239,11 +286,17 @@ static int kv_vec(const KvRows &r, int es, int unit) {
 #define KV_ROWS_LAUNCH(K, T, DD, QQ)                                                                       \
     do {                                                                                                   \
         const int vec = kv_vec(k, sizeof(T), DD / 16) && kv_vec(v, sizeof(T), DD / 16);                    \
-        hipLaunchKernelGGL((K<T, DD, QQ>), grid, dim3(KV_THREADS), 0, st, p, b, k, v, vec);                \
+        if (many) hipLaunchKernelGGL((K<T, DD, QQ, 4>), grid, dim3(KV_THREADS), 0, st, p, b, k, v, vec, lr, parts); \
+        else hipLaunchKernelGGL((K<T, DD, QQ, 1>), grid, dim3(KV_THREADS), 0, st, p, b, k, v, vec, lr, parts); \
     } while (0)
 #define KV_ROWS_DISPATCH(K)                                                                                \
-    const long long units = (long long)b.max_rows * p.hk * 2;                                              \
-    const long long blocks = (units + KV_THREADS / 16 - 1) / (KV_THREADS / 16);                            \
+    int lr = 0;                                                                                            \
+    while (lr < 4 && 1 << lr < b.max_rows) lr++;                                                           \
+    const long long groups = ((long long)b.max_rows + (1 << lr) - 1) >> lr;                                \
+    const long long step = KV_THREADS / 16 >> lr, singly = (2LL * p.hk + step - 1) / step;                 \
+    const bool many = groups * singly * b.n_seq > KV_ALL;                                                  \
+    const unsigned parts = (unsigned)(many ? (singly + 3) / 4 : singly);                                   \
+    const long long blocks = groups * parts;                                                               \
     if (blocks > INT_MAX) return -1;                                                                       \
     const dim3 grid((unsigned)blocks, b.n_seq);                                                            \
     if (p.d == 32) KV_ROWS_D(K, 32);                                                                       \

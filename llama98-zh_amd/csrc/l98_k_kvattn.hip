@@ -418,9 +418,21 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_kv_few(KvPages p, KvSeqs b, 
     __shared__ float sm[FEW_WAVES][ROWS], sl[FEW_WAVES][ROWS];
     static_assert(SC <= ROWS * D, "the scales fit");
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, h = lane >> 4;
-    // splits of a tile next to each other, the tiles with the most keys first
-    const int seq = blockIdx.y, split = blockIdx.x % w.splits, y = blockIdx.x / w.splits;
-    const int kh = y % p.hk, tile = tiles - 1 - y / p.hk;
+    // The later splits, which a short sequence does not have, come last: blocks
+    // are dealt to the CUs in turn, and with a sequence's splits next to each
+    // other some got three with keys and others none (32 sessions of 256 to
+    // 2048 keys: the median block took 13 us, the last 20).  Within a split the
+    // tiles with the most keys first.
+    int y = blockIdx.x;
+    const int seq = y % b.n_seq;
+    y /= b.n_seq;
+    const int kh = y % p.hk;
+    y /= p.hk;
+    const int tile = tiles - 1 - y % tiles, split = y / tiles;
+    const int k0 = split * chunk, step = FEW_WAVES * FEW_KEYS;
+    int key = k0 + wave * FEW_KEYS;
+    const int *table = b.table + seq * b.stride;
+    FewPages pg = few_pages(p, table, b.pages, key);         // (beside the lengths' loads)
     const KvSeq s = kv_seq(b, seq, p.shift);
     const int nr = s.n < b.max_rows ? s.n : b.max_rows;
     if ((long long)tile * ROWS >= (long long)nr * group) return;
@@ -429,10 +441,8 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_kv_few(KvPages p, KvSeqs b, 
     j_last = j_last < nr ? j_last : nr - 1;
     int end = s.pos0 + j_last + 1;                           // of the tile's keys
     end = end < s.len ? end : s.len;
-    const int k0 = split * chunk;
     int k1 = k0 + chunk;
     k1 = k1 < end ? k1 : end;
-    const int *table = b.table + seq * b.stride;
     if (k0 >= k1 && w.splits > 1) {                          // no keys: the join skips this part
         const int row = tile * ROWS + threadIdx.x, j = row / group, r = s.r0 + j;
         if (threadIdx.x < ROWS && j < nr && (unsigned)r < (unsigned)b.n_rows) {
@@ -444,11 +454,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_kv_few(KvPages p, KvSeqs b, 
 
     const FewAddr<D, Q8, BF> addr(p, kh);
     FewTile<D, Q8, BF> tl;
-    FewPages pg = {{-1, -1}};
-    const int step = FEW_WAVES * FEW_KEYS;
-    int key = k0 + wave * FEW_KEYS;
     if (key < k1) {
-        pg = few_pages(p, table, b.pages, key);
         addr.load_k(tl, p, pg, key);
         addr.load_v(tl, p, pg, key);
     }
@@ -662,6 +668,45 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_kv_join(KvSeqs b, KvRows out, 
     }
 }
 
+// The same for up to JOIN_FEW splits: one wave per (row, head), four of them
+// in a block.
+#define JOIN_FEW 16
+template <int D, bool BF>
+__global__ __launch_bounds__(256) void k_kv_join_few(KvSeqs b, KvRows out, int heads, KvParts w) {
+    using T = typename std::conditional<BF, __bf16, float>::type;
+    constexpr int E = D >= 64 ? D / 64 : 1;                  // dimensions of a lane
+    const long long x = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int j = (int)(x / heads), head = (int)(x % heads), seq = blockIdx.y, lane = threadIdx.x & 63;
+    const int r0 = b.row0[seq], nr = b.row0[seq + 1] - r0, r = r0 + j;
+    if (j >= nr || j >= b.max_rows || (unsigned)r >= (unsigned)b.n_rows) return;
+    const long long at = ((long long)r * heads + head) * w.splits;
+    const int d = lane * E < D ? lane * E : 0;
+    float o[JOIN_FEW][E];
+#pragma unroll
+    for (int i = 0; i < JOIN_FEW; i++)                       // (of a split without keys: of any content, not used)
+#pragma unroll
+        for (int e = 0; e < E; e++) o[i][e] = i < w.splits ? w.o[(at + i) * D + d + e] : 0.0f;
+    const float2 ml = lane < w.splits ? *(const float2 *)(w.ml + 2 * (at + lane)) : make_float2(ninf(), 0.0f);
+    float mx = ml.x;
+#pragma unroll
+    for (int y = 1; y < JOIN_FEW; y <<= 1) mx = fmaxf(mx, __shfl_xor(mx, y));
+    const float f = ml.x == ninf() ? 0.0f : kv_exp2(ml.x - mx);
+    float l = ml.x == ninf() ? 0.0f : ml.y * f, acc[E] = {};
+#pragma unroll
+    for (int y = 1; y < JOIN_FEW; y <<= 1) l += __shfl_xor(l, y);
+    l = __shfl(l, 0);
+#pragma unroll
+    for (int i = 0; i < JOIN_FEW; i++) {
+        const float g = __shfl(f, i), m = __shfl(ml.x, i);
+#pragma unroll
+        for (int e = 0; e < E; e++) acc[e] += m == ninf() ? 0.0f : o[i][e] * g;
+    }
+    if (lane * E >= D) return;
+    T *dst = (T *)out.p + r * out.row + head * out.head + d;
+#pragma unroll
+    for (int e = 0; e < E; e++) dst[e] = (T)(l == 0.0f ? 0.0f : acc[e] / l);
+}
+
 // ---------------------------------------------------------- host glue ---
 
 namespace {
@@ -672,21 +717,21 @@ KvPlan plan(const KvPages &p, const KvSeqs &b, int heads, int bf16) {
     KvPlan x;
     const long long rows = (long long)b.max_rows * (heads / p.hk);
     x.many = bf16 && rows > 128;
-    int unit, least;
-    long long want;
-    if (x.many) {
-        x.rows = (long long)b.n_seq * p.hk * ((rows + 255) / 256) >= 256 ? 256 : 128;
-        unit = 64;
-        least = 512;
-        want = 256;
-    } else {
-        x.rows = rows <= 16 ? 16 : 32;
-        unit = FEW_WAVES * FEW_KEYS;
-        least = 256;
-        want = 768;
-    }
+    // A block takes 512 keys or more: less costs more in starting and joining
+    // than it gives (300 keys of one session: 6.9 us in one block per head, 5.8
+    // and 3.1 for the join in two).
+    const int unit = x.many ? 64 : FEW_WAVES * FEW_KEYS, least = 512;
+    if (x.many) x.rows = (long long)b.n_seq * p.hk * ((rows + 255) / 256) >= 256 ? 256 : 128;
+    else x.rows = rows <= 16 ? 16 : 32;
     x.tiles = (int)((rows + x.rows - 1) / x.rows);
     const long long base = (long long)b.n_seq * p.hk * x.tiles;
+    // Blocks wanted: 256 of many rows, which have a CU each.  Of few rows two per
+    // CU for one sequence (8 rows at 250,015 keys: 256 blocks 72 us, 492 63, 980
+    // 74), but no splits where the tiles alone fill the chip (512 fp32 rows at
+    // 4096, 256 tiles: 77 us, with two splits 71 and 12 for the join); four for
+    // several, whose lengths differ (100 sessions of 1 to 5000 keys: 800 blocks
+    // 122 us, 1200 110, 2400 109).
+    const long long want = x.many ? 256 : b.n_seq > 1 ? 1024 : base >= 256 ? base : 512;
     long long splits = (want + base - 1) / base;
     const long long most = (b.max_len + least - 1) / least;
     splits = splits < most ? splits : most;
@@ -703,7 +748,7 @@ template <int D, bool Q8, bool BF>
 int few(const KvPages &p, const KvSeqs &b, const KvRows &q, const KvRows &o, int heads, float scale2, const KvPlan &x,
         const KvParts &w, hipStream_t st) {
     const int es = BF ? 2 : 4, vec = (uintptr_t)q.p % 16 == 0 && q.row * es % 16 == 0 && q.head * es % 16 == 0;
-    const dim3 grid((unsigned)((long long)x.splits * p.hk * x.tiles), b.n_seq);
+    const dim3 grid((unsigned)((long long)x.splits * p.hk * x.tiles * b.n_seq));
     if (x.rows == 16)
         hipLaunchKernelGGL((k_kv_few<D, Q8, BF, 1>), grid, dim3(FEW_THREADS), 0, st, p, b, q, o, heads, heads / p.hk,
                            scale2, x.chunk, x.tiles, vec, w);
@@ -722,7 +767,7 @@ int attend(const KvPages &p, int q8, const KvSeqs &b, const KvRows &q, const KvR
     w.o = (float *)((char *)ws + (x.many ? l98k_kv_many_ws(p, b) : 0));
     w.ml = w.o + (long long)b.n_rows * heads * x.splits * D;
     const float scale2 = scale * 1.44269504088896341f;
-    const long long blocks = (long long)x.splits * p.hk * x.tiles, joins = (long long)b.max_rows * heads;
+    const long long blocks = (long long)x.splits * p.hk * x.tiles * b.n_seq, joins = (long long)b.max_rows * heads;
     if (blocks > INT_MAX || joins > INT_MAX) return -1;
     int rc;
     if (x.many) rc = l98k_kv_many(p, q8, b, q, o, heads, scale2, x, w, ws, st);
@@ -731,8 +776,15 @@ int attend(const KvPages &p, int q8, const KvSeqs &b, const KvRows &q, const KvR
     else rc = bf16 ? few<D, false, true>(p, b, q, o, heads, scale2, x, w, st)
                    : few<D, false, false>(p, b, q, o, heads, scale2, x, w, st);
     if (rc || x.splits == 1) return rc;
-    if (bf16) hipLaunchKernelGGL((k_kv_join<D, true>), dim3((unsigned)joins, b.n_seq), dim3(JOIN_THREADS), 0, st, b, o, heads, w);
-    else hipLaunchKernelGGL((k_kv_join<D, false>), dim3((unsigned)joins, b.n_seq), dim3(JOIN_THREADS), 0, st, b, o, heads, w);
+#define JOIN_LAUNCH(K, BF, N) \
+    hipLaunchKernelGGL((K<D, BF>), dim3((unsigned)(N), b.n_seq), dim3(JOIN_THREADS), 0, st, b, o, heads, w)
+    if (x.splits <= JOIN_FEW) {
+        if (bf16) JOIN_LAUNCH(k_kv_join_few, true, (joins + 3) / 4);
+        else JOIN_LAUNCH(k_kv_join_few, false, (joins + 3) / 4);
+    } else {
+        if (bf16) JOIN_LAUNCH(k_kv_join, true, joins);
+        else JOIN_LAUNCH(k_kv_join, false, joins);
+    }
     return (int)hipGetLastError();
 }
 
