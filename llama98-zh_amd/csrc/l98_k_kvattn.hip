@@ -199,7 +199,9 @@ struct FewAcc {
     f32x4 o[MT][F::NT];
     float m[MT], l[MT], cq[MT];
     int lim[MT];                                             // the row's keys: below this
+    bool huge;                                               // some m is
 };
+__device__ __forceinline__ bool few_huge(float m) { return fabsf(m) > 0x1p20f && m != FEW_NONE; }
 
 // The scores of a tile, s[m][t][i] of query (lane & 15) and key t*16 + 4*(lane >> 4) + i.
 template <int D, bool Q8, bool BF, int MT>
@@ -310,7 +312,7 @@ __device__ __forceinline__ void few_values(FewAcc<D, Q8, BF, MT> &A, FewTile<D, 
         float mx = s[m][0][0];
 #pragma unroll
         for (int i = 1; i < 8; i++) mx = fmaxf(mx, s[m][i >> 2][i & 3]);
-        cand[m] = __builtin_fmaf(mx, A.cq[m], cand[m]);
+        cand[m] = mx * A.cq[m] + cand[m];                    // (rounded in two steps, as below)
         up = up || cand[m] > A.m[m] + ROOM;
     }
     if (__any(up)) {
@@ -325,14 +327,29 @@ __device__ __forceinline__ void few_values(FewAcc<D, Q8, BF, MT> &A, FewTile<D, 
 #pragma unroll
             for (int d = 0; d < F::NT; d++) A.o[m][d] *= f;
         }
+        bool any = false;
+#pragma unroll
+        for (int m = 0; m < MT; m++) any = any || few_huge(A.m[m]);
+        A.huge = __any(any);
     }
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+    for (int m = 0; m < MT; m++) {
+        float c = A.cq[m], mu = A.m[m];
+        // Of scores so large that the maximum's rounding is no small difference
+        // the products are rounded like it.
+        if (A.huge) {
+            const bool big = few_huge(mu);
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[m][i >> 2][i & 3] = big ? s[m][i >> 2][i & 3] * c - mu : s[m][i >> 2][i & 3];
+            c = big ? 1.0f : c;
+            mu = big ? 0.0f : mu;
+        }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            s[m][i >> 2][i & 3] = kv_exp2(__builtin_fmaf(s[m][i >> 2][i & 3], A.cq[m], -A.m[m]));
+            s[m][i >> 2][i & 3] = kv_exp2(__builtin_fmaf(s[m][i >> 2][i & 3], c, -mu));
             A.l[m] += s[m][i >> 2][i & 3];
         }
+    }
     if (!Q8 && masked) {
         // A key that some row may not attend must not reach it as 0 * NaN: its
         // V becomes zero; where it has a value that is not finite, the rows
@@ -468,6 +485,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_kv_few(KvPages p, KvSeqs b, 
         A.lim[m] = on ? (s.pos0 + j + 1 < s.len ? s.pos0 + j + 1 : s.len) : 0;
         A.m[m] = FEW_NONE;
         A.l[m] = 0.0f;
+        A.huge = false;
 #pragma unroll
         for (int d = 0; d < F::NT; d++) A.o[m][d] = f32x4{0, 0, 0, 0};
         float x[F::NG][8];
@@ -595,7 +613,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_kv_few(KvPages p, KvSeqs b, 
     }
     const long long at = ((long long)r * heads + head) * w.splits + split;
     if (d0 == 0) {
-        w.ml[2 * at] = mx == FEW_NONE ? ninf() : mx;
+        w.ml[2 * at] = mx == FEW_NONE && l == l ? ninf() : mx;   // (scores that are all NaN leave mx, and are not no keys)
         w.ml[2 * at + 1] = l;
     }
     if (mx != FEW_NONE)

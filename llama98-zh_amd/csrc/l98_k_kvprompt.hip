@@ -17,14 +17,16 @@
 // 12-15 of each 16.
 //
 // Q8 goes through fp16: q scaled per row by a power of two (exact for bf16), K
-// and V as code * scale * 2^(-9 - E) with E of the tile's largest scale (the
-// sums are rescaled when a larger one of V's comes): a byte u in an fp16's low bits is the
-// subnormal u 2^-24, and one packed fma, u 2^-24 * f - f 2^-17 with f the scale
-// times 2^(15 - E) rounded to fp16, makes the number of it.  Two roundings of
-// 2^-11, against the output's 2^-8; numbers below 2^-12 of the tile's largest
-// are held with a step of 2^-22 of it.  bf16 caches are used as they are.
-// Weights are rounded to the same 16 bits, and their sum, in fp32, is of the
-// rounded ones.
+// and V as code * (scale * 2^(8 - E)) with E of the tile's largest scale, so two
+// roundings of 2^-12 against the output's 2^-9 (the fp16 number 1024 + u is u
+// in the low bits of 1024's; less 1152 it is the code).  The sums are in units
+// of a V tile's 2^E, rescaled when a tile's is larger or less than 2^-4 of it.
+// Scales of down to 2^-22 of their tile's largest are held to full precision.
+// Where a tile has a wider range, or the tiles' V scales one of 2^60, the block
+// computes its rows again from the pages in fp32 (many_slowly): a key behind a
+// row may be of any size, and must not take the row's own out of the range.
+// bf16 caches are used as they are.  Weights are rounded to the same 16 bits,
+// and their sum, in fp32, is of the rounded ones.
 //
 // The running maximum is raised only where a tile exceeds it by 2^8 (weights
 // stay below 2^8): the sums are rescaled a few times per row instead of once
@@ -46,14 +48,6 @@ __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
 }
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ uint32_t times_2m17(uint32_t a) {         // of two fp16
-    f16x2 x;
-    __builtin_memcpy(&x, &a, 4);
-    x = x * (f16x2){(_Float16)-0x1p-17f, (_Float16)-0x1p-17f};
-    uint32_t r;
-    __builtin_memcpy(&r, &x, 4);
-    return r;
 }
 __device__ __forceinline__ float finite_or_0(float x) {
     return (u_from_f(x) & 0x7F800000u) == 0x7F800000u ? 0.0f : x;
@@ -174,39 +168,46 @@ __device__ __forceinline__ void many_scales(Stage<D, Q8, NT> &S, const KvPages &
     S.both[1] = *(const f32x4 *)(s + 16);
 }
 
-// Exponents above the tile's K and V scales, of the keys that exist.
+// Exponents above the tile's K and V scales, of the keys that exist, and
+// whether the smallest of K's or of V's is too small beside the largest.
+#define MANY_NONE (-126)                                     // no scale, or none above 2^-126
+#define MANY_RANGE 22
 template <int D, bool Q8, int NT>
-__device__ __forceinline__ void many_exps(Stage<D, Q8, NT> &S, uint32_t hole, int key, int len, int &ek, int &ev) {
+__device__ __forceinline__ void many_exps(Stage<D, Q8, NT> &S, uint32_t hole, int key, int len, int &ek, int &ev, bool &wide) {
     const int k = (threadIdx.x & 7) * 8;
+    uint32_t x = 0, y = 0;                                   // the largest, and the smallest above 0 taken from TOP
+    constexpr uint32_t TOP = 0x7F800000u;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const bool in = key + k + i < len && !(hole >> (k >> 4) & 1);
-        S.both[i >> 2][i & 3] = in ? finite_or_0(S.both[i >> 2][i & 3]) : 0.0f;
+        const uint32_t v = in ? u_from_f(fmaxf(finite_or_0(S.both[i >> 2][i & 3]), 0.0f)) : 0u, w = v ? TOP - v : 0u;
+        x = v > x ? v : x;
+        y = w > y ? w : y;
     }
-    float a = fmaxf(S.both[0][0], S.both[0][1]);
-#pragma unroll
-    for (int i = 2; i < 8; i++) a = fmaxf(a, S.both[i >> 2][i & 3]);
-    // the largest of each 32 lanes, in the last of them: by DPP, over rows of 16, then into the odd rows
-    uint32_t x = u_from_f(a);
-    auto step = [&](uint32_t y) { x = y > x ? y : x; };
-    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, true));   // row_shr:1
-    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, true));
-    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, true));
-    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, true));
-    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, true));   // row_bcast:15 into rows 1, 3
+    // over each 32 lanes, into the last of them: by DPP, over rows of 16, then into the odd rows
+    auto over = [](uint32_t &x) {
+        auto step = [&](uint32_t o) { x = o > x ? o : x; };
+        step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, true));   // row_shr:1
+        step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, true));
+        step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, true));
+        step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, true));
+        step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, true));   // row_bcast:15 into rows 1, 3
+    };
+    over(x);
+    over(y);
     ek = exp_above((uint32_t)__builtin_amdgcn_readlane((int)x, 31));
     ev = exp_above((uint32_t)__builtin_amdgcn_readlane((int)x, 63));
+    wide = ek - exp_above(TOP - (uint32_t)__builtin_amdgcn_readlane((int)y, 31)) > MANY_RANGE ||
+           ev - exp_above(TOP - (uint32_t)__builtin_amdgcn_readlane((int)y, 63)) > MANY_RANGE;
 }
 
-// bytes of lo and hi (sel: a byte of each over zeros), each minus 128, times
-// the scales' halves of f = 2^15 times what they are multiplied with; c = -f / 2^17
-__device__ __forceinline__ uint32_t scaled2(uint32_t hi, uint32_t lo, uint32_t sel, uint32_t f, uint32_t c) {
-    const uint32_t u = __builtin_amdgcn_perm(hi, lo, sel);   // as fp16: subnormals, u 2^-24
-    f16x2 x, y, z;
+// bytes of lo and hi (sel: a byte of each over zeros), each minus 128, times the halves of f
+__device__ __forceinline__ uint32_t scaled2(uint32_t hi, uint32_t lo, uint32_t sel, uint32_t f) {
+    const uint32_t u = __builtin_amdgcn_perm(hi, lo, sel) | 0x64006400u;     // as fp16: 1024 + u
+    f16x2 x, y;
     __builtin_memcpy(&x, &u, 4);
     __builtin_memcpy(&y, &f, 4);
-    __builtin_memcpy(&z, &c, 4);
-    x = __builtin_elementwise_fma(x, y, z);
+    x = (x - (f16x2){(_Float16)1152.0f, (_Float16)1152.0f}) * y;
     uint32_t r;
     __builtin_memcpy(&r, &x, 4);
     return r;
@@ -223,7 +224,8 @@ __device__ __forceinline__ int chunk_at(int r, int c) {
 struct ManyHead {
     int ek, ev;                                              // 2^these > every K and V scale of it
     uint32_t bad[2];                                         // keys whose V is not finite (it is zeros in the tile)
-    uint32_t hole, unused[3];                                // as ManyPages'
+    uint32_t hole;                                           // as ManyPages'
+    uint32_t wide, unused[2];                                // its scales' range is too wide for fp16
 };
 
 // The tile to k and v, and its keys whose V is not finite to bad (in LDS): a
@@ -241,13 +243,13 @@ __device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, uint16_t *kt, ui
         if (Q8) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float x = __builtin_amdgcn_ldexpf(S.ks[u][i], 15 - ek);
-                const uint32_t f = pack2<_Float16>(x, x), c2 = times_2m17(f);
+                const float x = __builtin_amdgcn_ldexpf(S.ks[u][i], 8 - ek);
+                const uint32_t f = pack2<_Float16>(x, x);
                 u32x4 o;
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
-                    o[2 * w] = scaled2(0, S.k[u][2 * i + w], 0x0c010c00u, f, c2);
-                    o[2 * w + 1] = scaled2(0, S.k[u][2 * i + w], 0x0c030c02u, f, c2);
+                    o[2 * w] = scaled2(0, S.k[u][2 * i + w], 0x0c010c00u, f);
+                    o[2 * w + 1] = scaled2(0, S.k[u][2 * i + w], 0x0c030c02u, f);
                 }
                 *(u32x4 *)&kt[chunk_at<D / 8>(k, 2 * c + i) * 8] = o;
             }
@@ -283,16 +285,15 @@ __device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, uint16_t *kt, ui
         }
         // the quad's place: 0-3, 8-11, 4-7, 12-15 of each 16 keys
         const int r = (k >> 2) & 3, slot = (k >> 4) * 16 + ((r & 1) * 2 + (r >> 1)) * 4;
-        uint32_t f[T::SG][2], f2[T::SG][2];
+        uint32_t f[T::SG][2];
         if (Q8) {
 #pragma unroll
             for (int g = 0; g < T::SG; g++)
 #pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    f[g][w] = pack2<_Float16>(__builtin_amdgcn_ldexpf(S.vs[u][g][2 * w], 15 - ev),
-                                              __builtin_amdgcn_ldexpf(S.vs[u][g][2 * w + 1], 15 - ev));
-                    f2[g][w] = times_2m17(f[g][w]);
-                }
+                for (int w = 0; w < 2; w++)
+                    f[g][w] = ev == MANY_NONE ? 0u
+                                              : pack2<_Float16>(__builtin_amdgcn_ldexpf(S.vs[u][g][2 * w], 8 - ev),
+                                                                __builtin_amdgcn_ldexpf(S.vs[u][g][2 * w + 1], 8 - ev));
         }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -303,8 +304,8 @@ __device__ __forceinline__ void many_store(Stage<D, Q8, NT> &S, uint16_t *kt, ui
                 dim = pos % (D / 16) * 16 + pos / (D / 16);
                 const int g = T::SG == 1 ? 0 : e >> 1;
                 const uint32_t sel = 0x0c040c00u + (uint32_t)e * 0x00010001u;
-                o.x = scaled2(S.v[u][1][0], S.v[u][0][0], sel, f[g][0], f2[g][0]);
-                o.y = scaled2(S.v[u][3][0], S.v[u][2][0], sel, f[g][1], f2[g][1]);
+                o.x = scaled2(S.v[u][1][0], S.v[u][0][0], sel, f[g][0]);
+                o.y = scaled2(S.v[u][3][0], S.v[u][2][0], sel, f[g][1]);
             } else {
                 dim = pos;
                 const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
@@ -337,12 +338,13 @@ __global__ __launch_bounds__(TILE_THREADS) void k_kv_tiles(KvPages p, KvSeqs b, 
     many_load<D, Q8, TILE_THREADS>(S, p, pg, kh, key);
     many_scales<D, Q8, TILE_THREADS>(S, p, pg, kh, key);
     int ek = 0, ev = 0;
-    if (Q8) many_exps<D, Q8, TILE_THREADS>(S, pg.hole, key, s.len, ek, ev);
+    bool wide = false;
+    if (Q8) many_exps<D, Q8, TILE_THREADS>(S, pg.hole, key, s.len, ek, ev, wide);
     uint16_t *out = (uint16_t *)tile_at<D>(ws, p.hk, seq, kh, n, tile);
     many_store<D, Q8, TILE_THREADS>(S, out, out + MANY_KEYS * D, bad, pg.hole, key, s.len, ek, ev);
     __syncthreads();
     if (threadIdx.x == 0) {
-        ManyHead h = {ek, ev, {bad[0], bad[1]}, pg.hole, {0, 0, 0}};
+        ManyHead h = {ek, ev, {bad[0], bad[1]}, pg.hole, wide, {0, 0}};
         heads[((long long)seq * p.hk + kh) * n + tile] = h;
     }
 }
@@ -353,6 +355,82 @@ typedef __attribute__((address_space(3))) void *many_lptr;
 // wave is here.
 template <int N> __device__ __forceinline__ void many_arrive() {
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// One row's keys k0 .. k1 - 1 by one wave, from the pages, in fp32: 64 keys at a
+// time, first a key to a lane for the scores, then D / 64 of V's bytes to a lane.
+// mem: D + 64 floats of the wave's own.  at: the row's part where the keys are split.
+template <int D>
+__device__ __noinline__ void many_slowly(KvPages p, const int *table, int pages, KvRows q, KvRows out, int r, int kh, int head,
+                                         float scale2, int k0, int k1, float *mem, KvParts w, long long at) {
+    constexpr int B = D >= 64 ? D / 64 : 1, G = D / 32;
+    const int lane = threadIdx.x & 63, b0 = lane * B < D ? lane * B : 0;
+    const uint32_t rows = 1u << p.shift;
+    const long long head0 = (long long)kh * rows * D, v0 = (long long)p.hk * rows * D, scales = 2 * v0;
+    auto dim_of = [](int byte) { return byte % (D / 16) * 16 + byte / (D / 16); };       // of V
+    float *const qs = mem, *const ps = mem + D;
+    const __bf16 *src = (const __bf16 *)q.p + r * q.row + head * q.head;
+    auto lanes = []() {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    lanes();
+    for (int d = lane; d < D; d += 64) qs[d] = (float)src[d];
+    float m = ninf(), l = 0.0f, acc[B] = {};
+    for (int key = k0; key < k1; key += 64) {
+        const int k = key + lane, page = k >> p.shift;
+        const int id = k < k1 && page < pages ? table[page] : -1;
+        const bool in = (unsigned)id < (unsigned)p.n_pages;
+        const unsigned char *base = p.data + (in ? id : 0) * p.page_bytes;
+        const uint32_t off = (uint32_t)k & (rows - 1);
+        lanes();
+        float x = 0.0f;
+        for (int g = 0; g < G; g++) {
+            float part = 0.0f;
+            for (int h = 0; h < 4; h++) {
+                const uint2 u = *(const uint2 *)(base + head0 + (long long)off * D + h * (D / 4) + g * 8);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    part = __builtin_fmaf((float)(int)(((i < 4 ? u.x : u.y) >> (8 * (i & 3))) & 255u) - 128.0f, qs[g * 32 + h * 8 + i], part);
+            }
+            x = __builtin_fmaf(part, *(const float *)(base + scales + (((long long)kh * G + g) * rows + off) * 4), x);
+        }
+        x = in ? x * scale2 : ninf();
+        float mx = x;
+        for (int i = 1; i < 64; i <<= 1) mx = fmaxf(mx, __shfl_xor(mx, i));
+        mx = fmaxf(mx, m);
+        const float f = m == ninf() ? 0.0f : kv_exp2(m - mx), pr = in ? kv_exp2(x - (mx == ninf() ? 0.0f : mx)) : 0.0f;
+        float sum = pr;
+        for (int i = 1; i < 64; i <<= 1) sum += __shfl_xor(sum, i);
+        l = l * f + sum;
+        m = mx;
+        ps[lane] = pr;
+        lanes();
+#pragma unroll
+        for (int i = 0; i < B; i++) acc[i] *= f;
+        for (int i = 0; i < 64; i++) {
+            const int vid = __shfl(id, i);
+            if ((unsigned)vid >= (unsigned)p.n_pages) continue;
+            const unsigned char *vb = p.data + vid * p.page_bytes;
+            const long long vo = (uint32_t)(key + i) & (rows - 1);
+            const float pi = ps[i];
+#pragma unroll
+            for (int e = 0; e < B; e++) {
+                const float c = (float)(int)vb[v0 + head0 + vo * D + b0 + e] - 128.0f;
+                const float sc = *(const float *)(vb + scales + (((long long)(p.hk + kh) * G + dim_of(b0 + e) / 32) * rows + vo) * 4);
+                acc[e] = __builtin_fmaf(pi, c * sc, acc[e]);
+            }
+        }
+    }
+    if (w.splits > 1 && lane == 0) *(float2 *)(w.ml + 2 * at) = make_float2(l == l ? m : fmaxf(m, -3.0e38f), l);
+    if (lane * B >= D) return;
+#pragma unroll
+    for (int e = 0; e < B; e++) {
+        const int d = dim_of(b0 + e);
+        if (w.splits > 1) w.o[at * D + d] = acc[e];
+        else ((__bf16 *)out.p)[r * out.row + head * out.head + d] = (__bf16)(l == 0.0f ? 0.0f : acc[e] / l);
+    }
 }
 
 template <int D, bool Q8, int NW>
@@ -417,7 +495,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
             const uint32_t o = __shfl_xor(big, 32);
             big = o > big ? o : big;
             e = (int)(big >> 23) - 127 - 14;
-            cq = __builtin_amdgcn_ldexpf(cq, e + 9);         // K comes with 2^(-9 - ek)
+            cq = __builtin_amdgcn_ldexpf(cq, e - 8);         // K comes with 2^(8 - ek)
         }
 #pragma unroll
         for (int c = 0; c < KK; c++)
@@ -427,7 +505,8 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
     f32x16 o[DT] = {}, st[2];
     u32x4 pw[2][2] = {};                                     // weights of the tile before
     float m = ninf(), l = 0.0f;
-    int ev = -1000;                                          // the unit's exponent of the sums
+    int ev = -1000, ev_least = 1000, ev_most = -1000;        // the unit's exponent of the sums; of all tiles
+    bool wide = false, huge = false;
 
     if (k0 < k1) {
         // Two halves of the block's waves, one of each on every SIMD, take turns:
@@ -454,6 +533,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
             x.bad[0] = a->bad[0];
             x.bad[1] = a->bad[1];
             x.hole = a->hole;
+            x.wide = a->wide;
             return x;
         };
         ManyHead head = head_of(0);
@@ -539,11 +619,16 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
                 const ManyHead hi = head;
                 head = head_of(i + 1);
                 const bool masked = key + MANY_KEYS > all || hi.hole || hi.bad[0] || hi.bad[1];
-                if (Q8 && hi.ev > ev) {                      // the sums' unit of V's scales grows
-                    const float f = __builtin_amdgcn_ldexpf(1.0f, ev - hi.ev);
+                if (Q8 && hi.ev != MANY_NONE) {
+                    if (hi.ev > ev || hi.ev < ev - 4) {      // the sums' unit changes
+                        const float f = __builtin_amdgcn_ldexpf(1.0f, ev - hi.ev);
 #pragma unroll
-                    for (int d = 0; d < DT; d++) o[d] *= f;
-                    ev = hi.ev;
+                        for (int d = 0; d < DT; d++) o[d] *= f;
+                        ev = hi.ev;
+                    }
+                    ev_least = hi.ev < ev_least ? hi.ev : ev_least;
+                    ev_most = hi.ev > ev_most ? hi.ev : ev_most;
+                    wide = wide || hi.wide;
                 }
                 float c = Q8 ? __builtin_amdgcn_ldexpf(cq, hi.ek) : cq;
                 c = fmaxf(c, 1e-37f);                        // -inf * c stays -inf at a scale of zero
@@ -576,9 +661,22 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
 #pragma unroll
                     for (int d = 0; d < DT; d++) o[d] *= f;
                     m = mn;
+                    huge = __any(fabsf(m) > 0x1p20f && m != ninf());
                 }
                 // weights in the sums' unit: V's tile has its own
-                const float less = Q8 ? (float)(ev - hi.ev) : 0.0f, mu = (m == ninf() ? 0.0f : m) + less;
+                const float less = Q8 && hi.ev != MANY_NONE ? (float)(ev - hi.ev) : 0.0f;
+                float mu = (m == ninf() ? 0.0f : m) + less;
+                // Of scores so large that the maximum's rounding is no small
+                // difference the products are rounded like it.
+                if (huge) {
+                    const bool mine = fabsf(m) > 0x1p20f && m != ninf();
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) st[t][e] = mine ? st[t][e] * c - m : st[t][e];
+                    c = mine ? 1.0f : c;
+                    mu = mine ? less : mu;
+                }
                 float sum = 0.0f;
 #pragma unroll
                 for (int t = 0; t < 2; t++)
@@ -598,11 +696,23 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
         }
         if (!g) asm volatile("s_barrier" ::: "memory");
         turn(c0(), cv(), n_tiles, []() {});
+        if (Q8 && (wide || ev_most - ev_least > 60)) {       // (of the whole block: its waves see the same tiles)
+            __syncthreads();
+            for (int i = 0; i < 32; i++) {
+                const int row = tile * ROWS + wave * 32 + i, j = row / group, r = s.r0 + j;
+                if (j >= nr || (unsigned)r >= (unsigned)b.n_rows) continue;
+                const int most = end_of(row);
+                many_slowly<D>(p, b.table + seq * b.stride, b.pages, q, out, r, kh, kh * group + row % group, scale2, k0,
+                               most < k1 ? most : k1, (float *)lk + wave * (D + 64), w,
+                               ((long long)r * heads + kh * group + row % group) * w.splits + split);
+            }
+            return;
+        }
     }
     l += __shfl_xor(l, 32);
     if (!on) return;
     if (Q8) {
-        const float f = __builtin_amdgcn_ldexpf(1.0f, ev == -1000 ? 0 : ev + 9);
+        const float f = __builtin_amdgcn_ldexpf(1.0f, ev == -1000 ? 0 : ev - 8);
 #pragma unroll
         for (int d = 0; d < DT; d++) o[d] *= f;
     }
@@ -628,7 +738,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
     }
     const long long at = ((long long)r * heads + head) * w.splits + split;
     if (h == 0) {
-        w.ml[2 * at] = m;
+        w.ml[2 * at] = l == l ? m : fmaxf(m, -3.0e38f);     // (scores that are all NaN leave m, and are not no keys)
         w.ml[2 * at + 1] = l;
     }
     if (m != ninf())

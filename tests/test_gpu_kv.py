@@ -171,7 +171,8 @@ class Problem:
                 r = (2 * ((self.dim + 16) * U + (H if bf and self.fmt == "q8" else 0)) * a + 2 * (n + 64) * U +
                      ((2 * B + H) if bf else 0))
                 out[self.row0[i]:self.row0[i + 1], h] = o
-                low = 2 * n * (2.0 ** -25 if bf and self.fmt == "q8" else 2.0 ** -38) * p.amax(1)[:, None] * vh.abs().max()
+                largest = torch.where(seen, vh.abs().amax(1), 0.0).amax(1)[:, None]      # of V that the row attends
+                low = 2 * n * (2.0 ** -25 if bf and self.fmt == "q8" else 2.0 ** -38) * p.amax(1)[:, None] * largest
                 tol[self.row0[i]:self.row0[i + 1], h] = (2 * r[:, None] * (p @ vh.abs()) + low +
                                                          ((B if bf else 0) + 2 * U) * o.abs())
         return out, tol
@@ -282,6 +283,90 @@ def test_nonfinite_rows_ahead(pkg, fmt, dt, lens):
             if w == 1 or not np.isinf(bad):        # a score of -inf or +inf may leave a finite row
                 assert not bool(torch.isfinite(out[before:p.n_rows]).all(-1).any())
             assert bool((out[p.n_rows:] == 77.0).all())
+
+
+BATCH = [(130, 130 + 37 * (i % 5)) if i % 4 else (i % 7 * 3, i % 7 * 11) for i in range(32)]
+
+
+@pytest.mark.parametrize("heads,hk,dim", [(16, 4, 128), (20, 4, 64), (4, 4, 32)])
+@pytest.mark.parametrize("fmt", ["q8", "bf16"])
+def test_attend_many_prompts(pkg, fmt, heads, hk, dim):
+    """Enough rows for a block of 256 each on every CU: batches of prompts of
+    odd lengths with empty ones and single rows between, and with holes."""
+    say("many prompts", fmt, heads, hk, dim)
+    lens = BATCH if heads > 4 else [(a * 4, n + 3 * a) for a, n in BATCH]
+    for page, holes in ((16, None), (64, {(3, 0): -1, (5, 1): 2 ** 31 - 1, (9, 2): 10 ** 6})):
+        p = Problem(pkg, fmt, "bf16", heads, hk, dim, page, lens, seed=page, holes=holes)
+        p.check(p.run())
+        assert torch.equal(p.run(), p.run())
+
+
+def test_attend_prompts_by_groups(pkg):
+    """A table and a bound of the lengths so large that the batch goes through
+    its workspace in two groups."""
+    say("groups")
+    lens = [(60, 60), (1, 900), (0, 0), (40, 700), (33, 34), (64, 300)]
+    p = Problem(pkg, "q8", "bf16", 16, 4, 128, 64, lens, seed=6)
+    table = torch.full((len(lens), 2048), -1, dtype=torch.int32, device=DEV)
+    table[:, :p.table.shape[1]] = p.table
+    p.batch = pkg.KvBatch(table, p.kv_len, p.row0_d, p.n_rows, p.max_rows, 131072)
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("fmt", ["q8", "bf16"])
+@pytest.mark.parametrize("lens", [[(8, 108)], [(150, 190)], [(150, 190)] * 64], ids=["few", "prompt", "prompts"])
+def test_huge_rows_ahead(pkg, fmt, lens):
+    """Finite K or V of 1e30 at a position, and from there on: a row before it
+    does not notice, one that attends it has what the formula says."""
+    for dt in ("f32", "bf16"):
+        rows, n = lens[0]
+        p = Problem(pkg, fmt, dt, 4, 2, 64, 16, lens, seed=3)
+        for at, to in ((n - rows // 2 - 1, n - rows // 2), (n - 5, n - 4), (n - rows // 2 - 1, n)):
+            for w in (0, 1):
+                say("huge", fmt, dt, lens[0], at, to, "KV"[w])
+                held = p.cache.bytes.copy(), [tuple(x.copy() for x in y) for y in p.kv]
+                r = np.random.default_rng(at)
+                for i in range(len(lens)):
+                    for a in range(at, to):
+                        kv = [x[a] for x in p.kv[i][:2]]
+                        kv[w] = r.standard_normal(kv[w].shape) * 1e30
+                        got = p.cache.put(int(p.table[i, a // 16]), a % 16, *kv)
+                        p.kv[i][w][a] = got[w]
+                p.check(p.run())
+                p.cache.bytes, p.kv = held
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("lens", [[(150, 560)], [(2, 560)]])
+def test_ranges_of_the_scales(pkg, dt, lens):
+    """Q8 values whose size changes from tile to tile and inside one, by 2^-20
+    to 2^20, up, down and to zero."""
+    for pattern in ([20, -20], [-20, 20], [0, -12, -6, 18, -18], [-20, None, 3], [-90, -60, -20]):
+        for run in (64, 16, 5):
+            say("ranges", dt, lens, pattern, run)
+            p = Problem(pkg, "q8", dt, 4, 2, 64, 16, lens, seed=run)
+            k, v, _ = p.kv[0]
+            for a in range(len(v)):
+                e = pattern[a // run % len(pattern)]
+                k[a], v[a] = p.cache.put(int(p.table[0, a // 16]), a % 16, k[a], v[a] * (0.0 if e is None else 2.0 ** e))
+            p.check(p.run())
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("fmt", ["q8", "bf16"])
+@pytest.mark.parametrize("lens", [[(2, 30000)], [(100, 9100)]])
+def test_nan_in_a_whole_split(pkg, fmt, dt, lens):
+    """Keys that are all NaN over more than a split's range reach every row."""
+    say("nan split", fmt, dt, lens)
+    p = Problem(pkg, fmt, dt, 8, 2, 64, 1024, lens, seed=4)
+    for page in range(1, 6):
+        blk = p.cache.bytes[int(p.table[0, page]), 0]
+        if fmt == "bf16":
+            blk.view(np.int16).reshape(2, 2, 1024, 64)[0, :, :, 7] = bf16(np.array([np.nan])).view(torch.int16).numpy()[0]
+        else:
+            blk[2 * 2 * 1024 * 64:].view(np.float32).reshape(2, 2, 2, 1024)[0, :, 1] = np.nan
+    out = p.run()
+    assert bool(out[:p.n_rows].isnan().all()) and bool((out[p.n_rows:] == 77.0).all())
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
@@ -398,6 +483,11 @@ def test_append_nonfinite(pkg):
     pool.read(p.batch, ko, vo)
     torch.cuda.synchronize()
     assert bool(ko[0, 0, :32].isnan().all()) and bool((ko[0, 0, 32:] == 1).all()) and bool((ko[1:] == 1).all())
+    assert bool((vo[1, 0, 32:] == 0).all()) and bool((vo[1, 0, :32] == 1).all()) and bool((vo[0] == 1).all())
+    v[1, 0, 32:] = torch.tensor([0x7FC00055, 0x7F800001], dtype=torch.int32, device=DEV).view(torch.float32).repeat(16)
+    pool.append(p.batch, k, v)                       # NaN with other bits
+    pool.read(p.batch, ko, vo)
+    torch.cuda.synchronize()
     assert bool((vo[1, 0, 32:] == 0).all()) and bool((vo[1, 0, :32] == 1).all()) and bool((vo[0] == 1).all())
 
 
