@@ -497,12 +497,21 @@ int l98_kv_read(const L98KvPool *pool, int layer, const L98KvBatch *b, const L98
 /* out[place][h] = sum_j p_j v_j / sum_j p_j over the positions j up to the
  * new row's own that exist, p_j = exp(scale * (q[place][h] . k_j)), K and V of
  * head h / (n_heads / n_kv_heads); a row with no such position gets zeros.
- * Softmax and sums in fp32.  A row never depends on positions behind its own,
- * whatever bits they hold; one that attends a row with infinities or NaN gets
- * such values.  n_heads: a multiple of n_kv_heads, at most 16 times it.  out
- * may be q.  ws: l98_kv_attend_ws_bytes bytes of device memory (NULL where
- * that is 0), 16-byte aligned, of any content, for this call alone until it
- * has run: calls or graphs that share it run one after the other. */
+ * Softmax and sums in fp32; bf16 rows' weights are rounded to 16 bits, and so
+ * are Q8 numbers where max_rows times a kv head's query heads is above 256.
+ * A row does not depend on positions behind its own: infinities and NaN there
+ * leave its bits as they are, finite numbers of another size may turn a
+ * rounding.  A row that attends infinities or NaN gets such values, in all of
+ * its dimensions or in some.  A row's bits may differ between calls of other
+ * bounds or batches, which split its keys otherwise; the same call gives the
+ * same bits.  n_heads: a multiple of n_kv_heads, at most 16 times it.  out may
+ * be q.  ws: l98_kv_attend_ws_bytes bytes of device memory (NULL where that is
+ * 0), 16-byte aligned, of any content, for this call alone until it has run:
+ * calls or graphs that share it run one after the other.  For prompts it holds
+ * their keys in the form that the matrix instructions take, 4 head_dim bytes
+ * per key and kv head, of as many sequences of max_len at a time as fit in
+ * 1 GiB (of one at least): a batch of prompts and one of single tokens are
+ * better two calls. */
 long long l98_kv_attend_ws_bytes(const L98KvPool *pool, const L98KvBatch *b, int n_heads, int dtype);
 int l98_kv_attend(const L98KvPool *pool, int layer, const L98KvBatch *b, const L98KvRows *q, const L98KvRows *out,
                   int n_heads, int dtype, float scale, void *ws, long long ws_bytes, void *stream, char *errbuf,

@@ -734,7 +734,11 @@ namespace {
 KvPlan plan(const KvPages &p, const KvSeqs &b, int heads, int bf16) {
     KvPlan x;
     const long long rows = (long long)b.max_rows * (heads / p.hk);
-    x.many = bf16 && rows > 128;
+    // The prompts' kernels from 257 rows on: with 256 (64 new rows of 4 heads, bf16
+    // cache) they take 31 us to these kernels' 19 for one sequence at 4000 keys,
+    // 36 to 36 for 8 at 1000, 61 to 56 for 32 at 1000, 225 to 170 for 32 at 4000;
+    // with 384 it is 32 to 26, 51 to 50, 70 to 83 and 243 to 255.
+    x.many = bf16 && rows > 256;
     // A block takes 512 keys or more: less costs more in starting and joining
     // than it gives (300 keys of one session: 6.9 us in one block per head, 5.8
     // and 3.1 for the join in two).
