@@ -5,7 +5,12 @@
 // `chunk` keys of one (sequence, kv head, tile of 16 MT rows), its four waves
 // 32 keys at a time in turn, and a second launch joins the blocks' partial
 // results where there is more than one per row.  A row of a tile is a (new
-// row, query head of the group) pair: m = new row * group + head.
+// row, query head of the group) pair: m = new row * group + head.  Measured
+// (16 heads over 4, width 128): 8 rows at 250,015 keys of Q8 64 us, 4.4 TB/s;
+// one row each of 100 sequences of 1 to 5000 keys in bf16 113 us, 4.7 TB/s; 4
+// fp32 rows each of 32 sequences of 256 to 2048 keys 18 us, of which a block's
+// start is a third.  512 fp32 rows at 4096 are bound by their registers and
+// vector instructions: 80 us.
 //
 // A wave computes S^T = K Q^T and O^T += V^T P^T with 16 x 16 x 32 matrix
 // instructions, so that the probabilities of a lane's S^T (query lane & 15,
@@ -19,10 +24,11 @@
 // scaled there.  q is scaled by a power of two per row to below 2^15; a bf16
 // row is then exact in fp16, an fp32 row goes as two fp16 parts (22 bits).
 // The weights w = p * (V's scale of the group) are at most 2^15 (the running
-// maximum is of s + log2(scale); the sum runs in the same unit), in one fp16 for bf16 rows (a rounding of 2^-11, against 2^-8 of the
-// output), two parts for fp32 rows.  bf16 caches: q and p in as many bf16
-// parts as their types need: a bf16 q is exact, fp32 takes three (24 bits); p
-// takes two for bf16 rows, three for fp32.
+// maximum is of s + log2(scale); the sum runs in the same unit), in one fp16
+// for bf16 rows (a rounding of 2^-12, against the output's 2^-9), two parts
+// for fp32 rows.  bf16 caches: q and p in as many bf16 parts as their types
+// need: a bf16 q is exact, fp32 takes three (24 bits); p takes two for bf16
+// rows, three for fp32.
 #include <limits.h>
 
 #include <type_traits>
@@ -750,7 +756,7 @@ KvPlan plan(const KvPages &p, const KvSeqs &b, int heads, int bf16) {
     // Blocks wanted: 256 of many rows, which have a CU each.  Of few rows two per
     // CU for one sequence (8 rows at 250,015 keys: 256 blocks 72 us, 492 63, 980
     // 74), but no splits where the tiles alone fill the chip (512 fp32 rows at
-    // 4096, 256 tiles: 77 us, with two splits 71 and 12 for the join); four for
+    // 4096, 256 tiles: 80 us, with two splits 74 and 12 for the join); four for
     // several, whose lengths differ (100 sessions of 1 to 5000 keys: 800 blocks
     // 122 us, 1200 110, 2400 109).
     const long long want = x.many ? 256 : b.n_seq > 1 ? 1024 : base >= 256 ? base : 512;
