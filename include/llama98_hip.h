@@ -467,7 +467,9 @@ typedef struct {
  * kv_len[i] - 1.  n_rows: the rows of those arrays; a place outside them is
  * left alone, and so are places that no sequence has.  max_rows and max_len:
  * bounds of a sequence's new rows and of kv_len, which size the launch; rows
- * and positions past them are left out.  n_seq <= 65535. */
+ * and positions past them are left out, and so are positions past the table
+ * (which is a bound of kv_len too; with both above 2^30 the call is refused).
+ * n_seq <= 65535. */
 typedef struct {
     const int *table;
     long long table_stride;
@@ -475,7 +477,9 @@ typedef struct {
     const int *kv_len, *row0;
     int n_seq, n_rows, max_rows, max_len;
 } L98KvBatch;
-/* Rows [place][head][dim] in device memory, strides in elements, dim's 1. */
+/* Rows [place][head][dim] in device memory, strides in elements, dim's 1.
+ * Rows that are written lie place after place or head after head, without
+ * overlaps; others may repeat (stride 0). */
 typedef struct {
     void *p;
     long long row_stride, head_stride;

@@ -742,6 +742,8 @@ class KvPool:
             raise ValueError(f"q is {q.dtype}, out is {out.dtype}")
         rq = _kv_rows(q, "q", batch.n_rows, 0, self.head_dim)
         ro = _kv_rows(out, "out", batch.n_rows, q.shape[1], self.head_dim)
+        if ws is not None and not ws.is_contiguous():
+            raise ValueError("ws is not contiguous")
         err = C.create_string_buffer(256)
         self._done(self.lib.l98_kv_attend(
             self.c, layer, batch.c, rq, ro, q.shape[1], code, scale, ws.data_ptr() if ws is not None else None,

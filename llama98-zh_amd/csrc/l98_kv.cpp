@@ -71,7 +71,7 @@ int host_pool(const L98KvPool *p, int layer, KvPages *out, char *errbuf, int err
     out->d = p->head_dim;
     return 0;
 }
-int host_batch(const L98KvBatch *b, KvSeqs *s, char *errbuf, int errlen) {
+int host_batch(const L98KvPool *p, const L98KvBatch *b, KvSeqs *s, char *errbuf, int errlen) {
     if (!b || b->n_seq < 0 || b->n_seq > 65535 || b->n_rows < 0 || b->max_rows < 0 || b->max_len < 0 ||
         b->table_pages < 0 || b->table_stride < 0)
         BAD("the batch is null or outside the limits");
@@ -83,7 +83,9 @@ int host_batch(const L98KvBatch *b, KvSeqs *s, char *errbuf, int errlen) {
     s->n_seq = b->n_seq;
     s->n_rows = b->n_rows;
     s->max_rows = std::min(b->max_rows, b->n_rows);
-    s->max_len = b->max_len;
+    // what a table can hold is a bound too; the kernels count keys, a chunk ahead, in 31 bits
+    s->max_len = (int)std::min<long long>(b->max_len, (long long)b->table_pages * p->page_rows);
+    if (s->max_len > 1 << 30) BAD("sequences of %d positions", s->max_len);
     return 0;
 }
 bool no_rows(const KvSeqs &s) { return s.n_seq == 0 || s.max_rows == 0; }
@@ -93,8 +95,12 @@ int host_rows(const L98KvRows *r, int dtype, int n_rows, int heads, int dim, boo
     if (!r) BAD("%s is null", name);
     if (dtype != L98_F32 && dtype != L98_BF16) BAD("dtype %d", dtype);
     if (r->row_stride < 0 || r->head_stride < 0) BAD("%s has a negative stride", name);
-    if (written && ((n_rows > 1 && r->row_stride < dim) || (heads > 1 && r->head_stride < dim)))
-        BAD("%s has rows or heads that overlap", name);
+    // one row's heads before the next, or one head's rows
+    const __int128 row = r->row_stride, head = r->head_stride;
+    if (written && !(n_rows <= 1 && (heads == 1 || head >= dim)) &&
+        !(row >= (heads - 1) * head + dim && (heads == 1 || head >= dim)) &&
+        !(head >= (n_rows - 1) * row + dim && row >= dim))
+        BAD("%s has rows or heads that overlap, or lie in each other", name);
     out->p = r->p;
     out->row = r->row_stride;
     out->head = r->head_stride;
@@ -146,7 +152,7 @@ int rows_call(RowsFn fn, bool written, const L98KvPool *pool, int layer, const L
     KvSeqs s;
     KvRows rk, rv;
     CHECK(host_pool(pool, layer, &p, errbuf, errlen));
-    CHECK(host_batch(b, &s, errbuf, errlen));
+    CHECK(host_batch(pool, b, &s, errbuf, errlen));
     CHECK(host_rows(k, dtype, s.n_rows, p.hk, p.d, written, "k", &rk, errbuf, errlen));
     CHECK(host_rows(v, dtype, s.n_rows, p.hk, p.d, written, "v", &rv, errbuf, errlen));
     if (no_rows(s)) return 0;
@@ -176,7 +182,7 @@ extern "C" int l98_kv_read(const L98KvPool *pool, int layer, const L98KvBatch *b
 extern "C" long long l98_kv_attend_ws_bytes(const L98KvPool *pool, const L98KvBatch *b, int n_heads, int dtype) {
     KvPages p = {};
     KvSeqs s;
-    if (host_pool(pool, 0, &p, nullptr, 0) || host_batch(b, &s, nullptr, 0) || host_heads(pool, n_heads, nullptr, 0) ||
+    if (host_pool(pool, 0, &p, nullptr, 0) || host_batch(pool, b, &s, nullptr, 0) || host_heads(pool, n_heads, nullptr, 0) ||
         (dtype != L98_F32 && dtype != L98_BF16))
         return -LZ_ERR_NULL_ARG;
     return no_rows(s) ? 0 : l98k_kv_attend_ws(p, pool->format == L98_KV_Q8, s, n_heads, dtype == L98_BF16);
@@ -191,11 +197,11 @@ extern "C" int l98_kv_attend(const L98KvPool *pool, int layer, const L98KvBatch 
     KvSeqs s;
     KvRows rq, ro;
     CHECK(host_pool(pool, layer, &p, errbuf, errlen));
-    CHECK(host_batch(b, &s, errbuf, errlen));
+    CHECK(host_batch(pool, b, &s, errbuf, errlen));
     CHECK(host_heads(pool, n_heads, errbuf, errlen));
     CHECK(host_rows(q, dtype, s.n_rows, n_heads, p.d, false, "q", &rq, errbuf, errlen));
     CHECK(host_rows(out, dtype, s.n_rows, n_heads, p.d, true, "out", &ro, errbuf, errlen));
-    if (!isfinite(scale)) BAD("scale is not finite");
+    if (!(fabsf(scale) < 1e38f)) BAD("scale is not finite, or above 1e38");
     if (no_rows(s)) return 0;
     const int q8 = pool->format == L98_KV_Q8, bf16 = dtype == L98_BF16;
     const long long need = l98k_kv_attend_ws(p, q8, s, n_heads, bf16);

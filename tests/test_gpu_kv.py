@@ -370,6 +370,37 @@ def test_nan_in_a_whole_split(pkg, fmt, dt, lens):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 90])
+def test_no_keys(pkg, dt, rows):
+    """A table of no pages, a bound of no positions, lengths of zero and below:
+    the rows are zeros, the others untouched; a bound without an end is the table's."""
+    say("no keys", dt, rows)
+    p = Problem(pkg, "q8", dt, 8, 2, 64, 16, [(rows, rows + 30), (0, 0), (rows, 2 * rows)], seed=rows)
+    pool = p.cache.pool()
+    full = p.run(pool)
+    none = torch.empty(3, 0, dtype=torch.int32, device=DEV)
+    for table, kv_len, max_len in ((none, p.kv_len, p.max_len), (p.table, p.kv_len, 0), (p.table, p.kv_len * 0, p.max_len),
+                                   (p.table, p.kv_len - 1000, p.max_len)):
+        p.batch = pkg.KvBatch(table, kv_len, p.row0_d, p.n_rows, p.max_rows, max_len)
+        out = torch.full_like(p.q, 77.0)
+        need = pool.attend_ws_bytes(p.batch, p.q)
+        pool.attend(p.batch, p.q, out, p.scale, torch.empty(need, dtype=torch.uint8, device=DEV) if need else None)
+        torch.cuda.synchronize()
+        assert bool((out[:p.n_rows] == 0).all()) and bool((out[p.n_rows:] == 77.0).all())
+        k = torch.full((p.n_rows, 2, 64), 5.0, device=DEV)
+        v = k.clone()
+        before = pool.data.clone()
+        pool.append(p.batch, k, v)
+        pool.read(p.batch, k, v)
+        torch.cuda.synchronize()
+        assert torch.equal(pool.data, before) and bool((k == 0).all()) and bool((v == 0).all())
+    p.batch = pkg.KvBatch(p.table, p.kv_len, p.row0_d, p.n_rows, p.max_rows, 2 ** 31 - 1)
+    p.check(p.run(pool))
+    with pytest.raises(ValueError, match="contiguous"):
+        pool.attend(p.batch, p.q, full, p.scale, torch.empty(1 << 20, 2, dtype=torch.uint8, device=DEV)[:, 0])
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("lens", [FEW, PROMPT])
 def test_strides_and_alignment(pkg, dt, lens):
     """q and out as slices of wider and of odd arrays, heads before rows, out

@@ -213,6 +213,32 @@ def test_calls_refuse(pkg):
         assert attend(b=big, dt=1, ws_bytes=need - 1) == NULL_ARG and b"workspace" in err.value
 
 
+def test_calls_refuse_sizes(pkg):
+    """Bounds that the kernels cannot count, scales beyond fp32, and written
+    rows and heads that lie in each other; layouts that do not are taken (they
+    get as far as the pointers, which are made up)."""
+    L = pkg.hip_lib()
+    err = C.create_string_buffer(200)
+    pool, ok = pool_of(pkg, n_pages=1 << 20), batch_of(pkg)
+
+    def attend(b=ok, out=None, scale=0.125):
+        return L.l98_kv_attend(pool, 0, b, rows_of(pkg, heads=8), out or rows_of(pkg, heads=8), 8, 0, scale, FAKE, 1 << 40,
+                               None, err, 200)
+
+    far = batch_of(pkg, max_len=2 ** 31 - 1, table_pages=1 << 27, table_stride=1 << 27)
+    assert attend(b=far) == NULL_ARG and b"positions" in err.value
+    assert L.l98_kv_attend_ws_bytes(pool, far, 8, 0) == NULL_ARG
+    lazy = batch_of(pkg, max_len=2 ** 31 - 1)             # the table's end is the bound
+    for dt in (0, 1):
+        assert L.l98_kv_attend_ws_bytes(pool, lazy, 8, dt) == L.l98_kv_attend_ws_bytes(pool, ok, 8, dt) >= 0
+    for scale in (1e38, -3e38):
+        assert attend(scale=scale) == NULL_ARG and b"scale" in err.value
+    for row, head in ((64, 64), (128, 64), (511, 64), (64, 383), (600, 100), (0, 512), (2 ** 62, 2 ** 62)):
+        assert attend(out=rows_of(pkg, row_stride=row, head_stride=head)) == NULL_ARG and b"overlap" in err.value, (row, head)
+    for row, head in ((512, 64), (64, 384), (1024, 128), (2 ** 61, 64), (128, 768)):
+        assert attend(out=rows_of(pkg, row_stride=row, head_stride=head)) != 0 and b"overlap" not in err.value, (row, head)
+
+
 def test_copy_refuses(pkg):
     L = pkg.hip_lib()
     err = C.create_string_buffer(200)
