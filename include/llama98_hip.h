@@ -502,7 +502,7 @@ int l98_kv_read(const L98KvPool *pool, int layer, const L98KvBatch *b, const L98
  * new row's own that exist, p_j = exp(scale * (q[place][h] . k_j)), K and V of
  * head h / (n_heads / n_kv_heads); a row with no such position gets zeros.
  * Softmax and sums in fp32; bf16 rows' weights are rounded to 16 bits, and so
- * are Q8 numbers where max_rows times a kv head's query heads is above 256.
+ * are Q8 numbers in batches of many rows (prompts).
  * A row does not depend on positions behind its own: infinities and NaN there
  * leave its bits as they are, finite numbers of another size may turn a
  * rounding.  A row that attends infinities or NaN gets such values, in all of

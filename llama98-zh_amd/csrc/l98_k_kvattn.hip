@@ -740,11 +740,15 @@ namespace {
 KvPlan plan(const KvPages &p, const KvSeqs &b, int heads, int bf16) {
     KvPlan x;
     const long long rows = (long long)b.max_rows * (heads / p.hk);
-    // The prompts' kernels from 257 rows on: with 256 (64 new rows of 4 heads, bf16
-    // cache) they take 31 us to these kernels' 19 for one sequence at 4000 keys,
-    // 36 to 36 for 8 at 1000, 61 to 56 for 32 at 1000, 225 to 170 for 32 at 4000;
-    // with 384 it is 32 to 26, 51 to 50, 70 to 83 and 243 to 255.
-    x.many = bf16 && rows > 256;
+    // The prompts' kernels where there is enough to do for their large blocks and
+    // two launches: above 256 rows, and 2^18 (32-row tile, key) pairs.  Measured
+    // (4 kv heads, Q8, width 128, few rows' kernels : prompts'): below, 128 new
+    // rows of 4 heads alone 11 : 17 us, 512 of them 17 : 27, 256 of them at 2000
+    // keys 33 : 37, 256 each of 4 sequences 17 : 21; above, 384 at 2000 keys 46 :
+    // 39, 384 each of 4 sequences 27 : 25, 512 each 36 : 29, at 2000 keys 108 : 89;
+    // 64 new rows of 32 sequences at 4000 keys (256 rows) 175 : 239.
+    const long long few = (long long)b.n_seq * p.hk * ((rows + 31) / 32);
+    x.many = bf16 && rows > 256 && (double)few * b.max_len > 262144.0;
     // A block takes 512 keys or more: less costs more in starting and joining
     // than it gives (300 keys of one session: 6.9 us in one block per head, 5.8
     // and 3.1 for the join in two).

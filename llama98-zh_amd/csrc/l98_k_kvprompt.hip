@@ -462,6 +462,25 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
     const int end = end_of(tile * ROWS + ROWS - 1), all = end_of(tile * ROWS);
     k1 = k1 < end ? k1 : end;
 
+    // The first tiles' loads go ahead of everything else.
+    const int n_tiles = (k1 - k0 + MANY_KEYS - 1) / MANY_KEYS, t0 = k0 / MANY_KEYS;
+    constexpr int LOADS = TILE * 2 / 1024, PER = 2 * LOADS / NW;         // of 1 KB, of K; a wave's
+    const unsigned char *src = tile_at<D>(ws, p.hk, seq, kh, per_seq, t0) + wave * PER * 1024;
+    auto load = [&](int i) {                             // tile i (the last one again behind the end)
+        const unsigned char *a = src + (long long)(i < n_tiles ? i : n_tiles - 1) * (4 * TILE) + lane * 16;
+        char *k = (char *)(lk + i % 3 * TILE), *v = (char *)(lv + (i & 3) * TILE);
+#pragma unroll
+        for (int e = 0; e < PER; e++) {
+            const int x = wave * PER + e;
+            __builtin_amdgcn_global_load_lds((many_gptr)(a + e * 1024),
+                                             (many_lptr)(x < LOADS ? k + x * 1024 : v + (x - LOADS) * 1024), 16, 0, 0);
+        }
+    };
+    if (k0 < k1) {
+        load(0);
+        load(1);
+    }
+
     const int row = tile * ROWS + wave * 32 + n, j = row / group, head = kh * group + row % group, r = s.r0 + j;
     const bool on = j < nr && (unsigned)r < (unsigned)b.n_rows;
     const int lim = on ? end_of(row) : 0;
@@ -469,6 +488,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
     float cq = fabsf(scale2);
     V8 qf[KK];
     {
+        // (a row that is not reads another's: a guard around each load would make them wait for each other)
         const __bf16 *src = (const __bf16 *)q.p + (on ? r * q.row + head * q.head : 0);
         float x[KK][8];
         uint32_t big = 0;
@@ -478,10 +498,10 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
             const int d0 = Q8 ? (at % (D / 32)) * 32 + at / (D / 32) * 8 : at * 8;
             bf16x8 t;
             if (vec) {
-                t = on ? *(const bf16x8 *)(src + d0) : bf16x8{};
+                t = *(const bf16x8 *)(src + d0);
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; i++) t[i] = on ? src[d0 + i] : (__bf16)0.0f;
+                for (int i = 0; i < 8; i++) t[i] = src[d0 + i];
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -519,9 +539,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
         // 2 j - 1, K's readers are in slots 2 j and 2 j + 1, V's in 2 j + 2 and
         // 2 j + 3: three buffers for K and four for V.
         // (Four waves, of small calls, have a SIMD each: they are all half 0.)
-        const int g = NW == 8 ? wave / 4 : 0, n_tiles = (k1 - k0 + MANY_KEYS - 1) / MANY_KEYS, t0 = k0 / MANY_KEYS;
-        constexpr int LOADS = TILE * 2 / 1024, PER = 2 * LOADS / NW;         // of 1 KB, of K; a wave's
-        const unsigned char *src = tile_at<D>(ws, p.hk, seq, kh, per_seq, t0) + wave * PER * 1024;
+        const int g = NW == 8 ? wave / 4 : 0;
         // (constant memory to this launch: scalar loads, a tile ahead)
         typedef const __attribute__((address_space(4))) ManyHead *head_ptr;
         const head_ptr hds = (head_ptr)(uintptr_t)(hd + (((long long)seq * p.hk + kh) * per_seq + t0));
@@ -537,18 +555,6 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
             return x;
         };
         ManyHead head = head_of(0);
-        auto load = [&](int i) {                             // tile i (the last one again behind the end)
-            const unsigned char *a = src + (long long)(i < n_tiles ? i : n_tiles - 1) * (4 * TILE) + lane * 16;
-            char *k = (char *)(lk + i % 3 * TILE), *v = (char *)(lv + (i & 3) * TILE);
-#pragma unroll
-            for (int e = 0; e < PER; e++) {
-                const int x = wave * PER + e;
-                __builtin_amdgcn_global_load_lds((many_gptr)(a + e * 1024),
-                                                 (many_lptr)(x < LOADS ? k + x * 1024 : v + (x - LOADS) * 1024), 16, 0, 0);
-            }
-        };
-        load(0);
-        load(1);
         // the first turn's values are of a tile that is not: no weights, and numbers to take them times
         for (int x = threadIdx.x; x < TILE / 8; x += NW * 64) ((u32x4 *)(lv + 3 * TILE))[x] = u32x4{0, 0, 0, 0};
         __syncthreads();

@@ -224,7 +224,8 @@ def test_attend(pkg, fmt, dt, heads, hk, dim):
 def test_attend_long(pkg, fmt, dt):
     """Contexts that are split: one sequence among short ones, and long
     prefixes before a chunk of rows."""
-    for lens, page in (([(3, 40011), (1, 17), (8, 9000)], 128), ([(100, 9100)], 64), ([(20, 20000), (33, 33)], 32)):
+    for lens, page in (([(3, 40011), (1, 17), (8, 9000)], 128), ([(100, 9100)], 64), ([(20, 20000), (33, 33)], 32),
+                       ([(150, 9100), (1, 5)], 64)):
         say("long", fmt, dt, lens)
         p = Problem(pkg, fmt, dt, 8, 2, 64, page, lens, seed=len(lens))
         p.check(p.run())
@@ -234,7 +235,8 @@ def test_attend_long(pkg, fmt, dt):
 def test_attend_scales(pkg, sharp):
     """A scale of zero (the mean), negative, and so large that one key takes all."""
     for fmt, dt, lens in (("q8", "bf16", [(90, 300)]), ("bf16", "f32", [(4, 300)]), ("q8", "f32", [(4, 900), (64, 64)]),
-                          ("bf16", "bf16", [(3, 1000), (200, 200)])):
+                          ("bf16", "bf16", [(3, 1000), (200, 200)]), ("q8", "bf16", [(1300, 1300), (64, 64)]),
+                          ("bf16", "bf16", [(1300, 1300), (64, 64)])):
         say("scale", sharp, fmt, dt, lens)
         p = Problem(pkg, fmt, dt, 4, 1, 64, 16, lens, seed=5, sharp=sharp)
         p.check(p.run())
@@ -257,7 +259,7 @@ def test_holes(pkg, fmt, dt):
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("fmt", ["q8", "bf16"])
-@pytest.mark.parametrize("lens", [[(8, 108)], [(150, 190)]])
+@pytest.mark.parametrize("lens", [[(8, 108)], [(150, 190)], [(2000, 2040)]])
 def test_nonfinite_rows_ahead(pkg, fmt, dt, lens):
     """Infinities and NaN in K and V at a position: the rows before it are
     what they are without it, bit for bit, the rows that attend it are not finite."""
@@ -288,6 +290,18 @@ def test_nonfinite_rows_ahead(pkg, fmt, dt, lens):
 BATCH = [(130, 130 + 37 * (i % 5)) if i % 4 else (i % 7 * 3, i % 7 * 11) for i in range(32)]
 
 
+@pytest.mark.parametrize("heads,hk,dim,lens", [(16, 4, 32, PROMPT), (20, 4, 64, PROMPT), (28, 4, 128, PROMPT),
+                                               (8, 8, 64, [(600, 640), (1, 700), (513, 513), (5, 9)]),
+                                               (7, 1, 128, [(300, 3000), (1, 1), (130, 2500)])])
+@pytest.mark.parametrize("fmt", ["q8", "bf16"])
+def test_attend_some_prompts(pkg, fmt, heads, hk, dim, lens):
+    """Prompts that are few, in blocks of 128 rows: whole and split, odd groups."""
+    say("some prompts", fmt, heads, hk, dim, lens)
+    for page in (16, 128):
+        p = Problem(pkg, fmt, "bf16", heads, hk, dim, page, lens, seed=page)
+        p.check(p.run())
+
+
 @pytest.mark.parametrize("heads,hk,dim", [(16, 4, 128), (20, 4, 64), (4, 4, 32)])
 @pytest.mark.parametrize("fmt", ["q8", "bf16"])
 def test_attend_many_prompts(pkg, fmt, heads, hk, dim):
@@ -305,7 +319,7 @@ def test_attend_prompts_by_groups(pkg):
     """A table and a bound of the lengths so large that the batch goes through
     its workspace in two groups."""
     say("groups")
-    lens = [(60, 60), (1, 900), (0, 0), (40, 700), (33, 34), (64, 300)]
+    lens = [(60, 60), (1, 900), (0, 0), (40, 700), (33, 34), (70, 300)]
     p = Problem(pkg, "q8", "bf16", 16, 4, 128, 64, lens, seed=6)
     table = torch.full((len(lens), 2048), -1, dtype=torch.int32, device=DEV)
     table[:, :p.table.shape[1]] = p.table
@@ -314,7 +328,8 @@ def test_attend_prompts_by_groups(pkg):
 
 
 @pytest.mark.parametrize("fmt", ["q8", "bf16"])
-@pytest.mark.parametrize("lens", [[(8, 108)], [(150, 190)], [(150, 190)] * 64], ids=["few", "prompt", "prompts"])
+@pytest.mark.parametrize("lens", [[(8, 108)], [(150, 190)], [(150, 190)] * 80, [(2000, 2040)]],
+                         ids=["few", "prompt", "prompts", "long prompt"])
 def test_huge_rows_ahead(pkg, fmt, lens):
     """Finite K or V of 1e30 at a position, and from there on: a row before it
     does not notice, one that attends it has what the formula says."""
@@ -337,7 +352,7 @@ def test_huge_rows_ahead(pkg, fmt, lens):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
-@pytest.mark.parametrize("lens", [[(150, 560)], [(2, 560)]])
+@pytest.mark.parametrize("lens", [[(150, 560)], [(2, 560)], [(1500, 1560)]])
 def test_ranges_of_the_scales(pkg, dt, lens):
     """Q8 values whose size changes from tile to tile and inside one, by 2^-20
     to 2^20, up, down and to zero."""
@@ -354,7 +369,7 @@ def test_ranges_of_the_scales(pkg, dt, lens):
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("fmt", ["q8", "bf16"])
-@pytest.mark.parametrize("lens", [[(2, 30000)], [(100, 9100)]])
+@pytest.mark.parametrize("lens", [[(2, 30000)], [(100, 9100)], [(150, 9100)]])
 def test_nan_in_a_whole_split(pkg, fmt, dt, lens):
     """Keys that are all NaN over more than a split's range reach every row."""
     say("nan split", fmt, dt, lens)
@@ -401,7 +416,7 @@ def test_no_keys(pkg, dt, rows):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
-@pytest.mark.parametrize("lens", [FEW, PROMPT])
+@pytest.mark.parametrize("lens", [FEW, PROMPT, PROMPT * 2])
 def test_strides_and_alignment(pkg, dt, lens):
     """q and out as slices of wider and of odd arrays, heads before rows, out
     in q's place: the same bits as the contiguous call's."""
@@ -556,6 +571,10 @@ def test_far_pages(pkg):
         for k in range((2, 4)[i]):
             t[int(table[i, k])] = torch.from_numpy(p.cache.bytes[int(p.table[i, k])].reshape(-1)).to(DEV)
     p.batch = pkg.KvBatch(table, p.kv_len, p.row0_d, p.n_rows, p.max_rows, p.max_len)
+    p.check(p.run(pool))
+    wide = torch.full((2, 64), -1, dtype=torch.int32, device=DEV)
+    wide[:, :4] = table
+    p.batch = pkg.KvBatch(wide, p.kv_len, p.row0_d, p.n_rows, p.max_rows, 4096)      # as prompts
     p.check(p.run(pool))
     pool.copy_pages([far[2], far[3]], [7, far[0] - 6])
     torch.cuda.synchronize()
