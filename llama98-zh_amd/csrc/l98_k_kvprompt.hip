@@ -9,6 +9,10 @@
 // with the conversion in the second kernel its waves issued 230 vector and 87
 // scalar instructions per tile beside the 32 matrix ones, and took 1.23 ms).
 //
+// The tiles too are put together in LDS and stored from there in 16-byte pieces
+// (V's 8-byte pieces of 64 rows a store straight to memory: 24,752 keys 27 us, so
+// 18, and 17 and 13 for 16,384; the floors are 15 and 10).
+//
 // k_kv_many: the bound is the matrix cores.  A block takes 32 NW rows of one
 // (sequence, kv head), 32 for each of its waves, and all waves share the tiles,
 // which are loaded straight into LDS two tiles ahead.  S^T = K Q^T and O^T += V^T
@@ -328,6 +332,7 @@ __device__ __forceinline__ unsigned char *tile_at(unsigned char *ws, int hk, int
 template <int D, bool Q8>
 __global__ __launch_bounds__(TILE_THREADS) void k_kv_tiles(KvPages p, KvSeqs b, int n, unsigned char *ws, ManyHead *heads) {
     __shared__ uint32_t bad[2];
+    __shared__ __align__(16) uint16_t made[2 * MANY_KEYS * D];
     const int seq = blockIdx.y, kh = blockIdx.x % p.hk, tile = blockIdx.x / p.hk, key = tile * MANY_KEYS;
     const KvSeq s = kv_seq(b, seq, p.shift);
     if (key >= s.len || s.n <= 0) return;
@@ -340,9 +345,12 @@ __global__ __launch_bounds__(TILE_THREADS) void k_kv_tiles(KvPages p, KvSeqs b, 
     int ek = 0, ev = 0;
     bool wide = false;
     if (Q8) many_exps<D, Q8, TILE_THREADS>(S, pg.hole, key, s.len, ek, ev, wide);
-    uint16_t *out = (uint16_t *)tile_at<D>(ws, p.hk, seq, kh, n, tile);
-    many_store<D, Q8, TILE_THREADS>(S, out, out + MANY_KEYS * D, bad, pg.hole, key, s.len, ek, ev);
+    many_store<D, Q8, TILE_THREADS>(S, made, made + MANY_KEYS * D, bad, pg.hole, key, s.len, ek, ev);
     __syncthreads();
+    u32x4 *out = (u32x4 *)tile_at<D>(ws, p.hk, seq, kh, n, tile);
+#pragma unroll
+    for (int i = 0; i < 4 * MANY_KEYS * D / 16 / TILE_THREADS; i++)
+        out[i * TILE_THREADS + threadIdx.x] = ((const u32x4 *)made)[i * TILE_THREADS + threadIdx.x];
     if (threadIdx.x == 0) {
         ManyHead h = {ek, ev, {bad[0], bad[1]}, pg.hole, wide, {0, 0}};
         heads[((long long)seq * p.hk + kh) * n + tile] = h;
@@ -716,32 +724,49 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
         }
     }
     l += __shfl_xor(l, 32);
-    if (!on) return;
     if (Q8) {
         const float f = __builtin_amdgcn_ldexpf(1.0f, ev == -1000 ? 0 : ev - 8);
 #pragma unroll
         for (int d = 0; d < DT; d++) o[d] *= f;
     }
     if (w.splits == 1) {
-        __bf16 *dst = (__bf16 *)out.p + r * out.row + head * out.head;
+        // Through LDS, so that a wave's stores are of whole rows (as the lanes have
+        // them, 8 bytes of each of 32 rows: nine packed prompts 419 us, so 411).
+        constexpr int CH = D / 8;                            // 16-byte chunks of a row
+        __syncthreads();                                     // the other waves' last turn
+        uint16_t *const mine = lv + wave * (32 * D);
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
-                const int d0 = d * 32 + (i >> 2) * 8 + h * 4;
+                const int c = d * 4 + (i >> 2);
                 uint2 t;
                 t.x = pack2<__bf16>(o[d][i] * inv, o[d][i + 1] * inv);
                 t.y = pack2<__bf16>(o[d][i + 2] * inv, o[d][i + 3] * inv);
-                if (vec) {
-                    *(uint2 *)(dst + d0) = t;
-                } else {
-                    uint16_t *x = (uint16_t *)dst + d0;
-                    x[0] = (uint16_t)t.x, x[1] = (uint16_t)(t.x >> 16), x[2] = (uint16_t)t.y, x[3] = (uint16_t)(t.y >> 16);
-                }
+                *(uint2 *)(mine + n * D + (c ^ (n & (CH - 1))) * 8 + h * 4) = t;
             }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        const long long at = on ? r * out.row + head * out.head : -1;
+#pragma unroll
+        for (int i = 0; i < CH / 2; i++) {
+            const int x = i * 64 + lane, m = x / CH, c = x % CH;
+            const u32x4 t = *(const u32x4 *)(mine + m * D + (c ^ (m & (CH - 1))) * 8);
+            const long long to = __shfl(at, m);
+            if (to < 0) continue;
+            uint16_t *dst = (uint16_t *)out.p + to + c * 8;
+            if (vec) {
+                *(u32x4 *)dst = t;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) dst[e] = (uint16_t)(t[e / 2] >> (16 * (e & 1)));
+            }
+        }
         return;
     }
+    if (!on) return;
     const long long at = ((long long)r * heads + head) * w.splits + split;
     if (h == 0) {
         w.ml[2 * at] = l == l ? m : fmaxf(m, -3.0e38f);     // (scores that are all NaN leave m, and are not no keys)
