@@ -13,7 +13,9 @@
 // (V's 8-byte pieces of 64 rows a store straight to memory: 24,752 keys 27 us, so
 // 18, and 17 and 13 for 16,384; the floors are 15 and 10).
 //
-// k_kv_many: the bound is the matrix cores.  A block takes 32 NW rows of one
+// k_kv_many: the bound is the matrix cores (a 16,384-token prompt, 16 heads over
+// 4 of width 128, Q8: 1.10 ms, 1.0 PFLOP/s; the matrix cores are busy in 48% of
+// its cycles, at the 2.0 GHz that the power limit leaves).  A block takes 32 NW rows of one
 // (sequence, kv head), 32 for each of its waves, and all waves share the tiles,
 // which are loaded straight into LDS two tiles ahead.  S^T = K Q^T and O^T += V^T
 // P^T by 32 x 32 x 16 instructions: a lane's S^T (query lane & 31) is the second
@@ -25,10 +27,13 @@
 // roundings of 2^-12 against the output's 2^-9 (the fp16 number 1024 + u is u
 // in the low bits of 1024's; less 1152 it is the code).  The sums are in units
 // of a V tile's 2^E, rescaled when a tile's is larger or less than 2^-4 of it.
-// Scales of down to 2^-22 of their tile's largest are held to full precision.
-// Where a tile has a wider range, or the tiles' V scales one of 2^60, the block
-// computes its rows again from the pages in fp32 (many_slowly): a key behind a
-// row may be of any size, and must not take the row's own out of the range.
+// Scales of down to 2^-22 of their tile's largest are held to full precision,
+// smaller ones with an error of 2^-33 of it.  A key behind a row may be of any
+// size, and must not take the row's own out of the range: where a tile that
+// some row attends in part has a V so much larger than its first key's, where
+// the error of K's numbers would show in the scores, and where the tiles' V
+// scales differ by 2^60, the block computes its rows again from the pages in
+// fp32 (many_slowly: 4096 rows of which all do take 36 ms instead of 0.15).
 // bf16 caches are used as they are.  Weights are rounded to the same 16 bits,
 // and their sum, in fp32, is of the rounded ones.
 //
@@ -173,18 +178,22 @@ __device__ __forceinline__ void many_scales(Stage<D, Q8, NT> &S, const KvPages &
 }
 
 // Exponents above the tile's K and V scales, of the keys that exist, and
-// whether the smallest of K's or of V's is too small beside the largest.
+// whether fp16 numbers of that unit are too coarse: bit 0, for the smallest
+// scale of K; bit 1, for the first key's of V (a row that attends some of the
+// tile attends that one, so what it attends is no smaller).
 #define MANY_NONE (-126)                                     // no scale, or none above 2^-126
 #define MANY_RANGE 22
 template <int D, bool Q8, int NT>
-__device__ __forceinline__ void many_exps(Stage<D, Q8, NT> &S, uint32_t hole, int key, int len, int &ek, int &ev, bool &wide) {
+__device__ __forceinline__ void many_exps(Stage<D, Q8, NT> &S, uint32_t hole, int key, int len, int &ek, int &ev, uint32_t &wide) {
     const int k = (threadIdx.x & 7) * 8;
     uint32_t x = 0, y = 0;                                   // the largest, and the smallest above 0 taken from TOP
     constexpr uint32_t TOP = 0x7F800000u;
+    const int first = (__ffs((int)~hole) - 1) * 16;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const bool in = key + k + i < len && !(hole >> (k >> 4) & 1);
-        const uint32_t v = in ? u_from_f(fmaxf(finite_or_0(S.both[i >> 2][i & 3]), 0.0f)) : 0u, w = v ? TOP - v : 0u;
+        const uint32_t v = in ? u_from_f(fmaxf(finite_or_0(S.both[i >> 2][i & 3]), 0.0f)) : 0u;
+        const uint32_t w = v && (!(threadIdx.x & 32) || k + i == first) ? TOP - v : 0u;
         x = v > x ? v : x;
         y = w > y ? w : y;
     }
@@ -201,8 +210,9 @@ __device__ __forceinline__ void many_exps(Stage<D, Q8, NT> &S, uint32_t hole, in
     over(y);
     ek = exp_above((uint32_t)__builtin_amdgcn_readlane((int)x, 31));
     ev = exp_above((uint32_t)__builtin_amdgcn_readlane((int)x, 63));
-    wide = ek - exp_above(TOP - (uint32_t)__builtin_amdgcn_readlane((int)y, 31)) > MANY_RANGE ||
-           ev - exp_above(TOP - (uint32_t)__builtin_amdgcn_readlane((int)y, 63)) > MANY_RANGE;
+    const int lk = exp_above(TOP - (uint32_t)__builtin_amdgcn_readlane((int)y, 31));
+    const int lv = exp_above(TOP - (uint32_t)__builtin_amdgcn_readlane((int)y, 63));
+    wide = (ek - lk > MANY_RANGE ? 1u : 0u) | (ev - lv > MANY_RANGE ? 2u : 0u);
 }
 
 // bytes of lo and hi (sel: a byte of each over zeros), each minus 128, times the halves of f
@@ -229,7 +239,7 @@ struct ManyHead {
     int ek, ev;                                              // 2^these > every K and V scale of it
     uint32_t bad[2];                                         // keys whose V is not finite (it is zeros in the tile)
     uint32_t hole;                                           // as ManyPages'
-    uint32_t wide, unused[2];                                // its scales' range is too wide for fp16
+    uint32_t wide, unused[2];                                // many_exps'
 };
 
 // The tile to k and v, and its keys whose V is not finite to bad (in LDS): a
@@ -343,7 +353,7 @@ __global__ __launch_bounds__(TILE_THREADS) void k_kv_tiles(KvPages p, KvSeqs b, 
     many_load<D, Q8, TILE_THREADS>(S, p, pg, kh, key);
     many_scales<D, Q8, TILE_THREADS>(S, p, pg, kh, key);
     int ek = 0, ev = 0;
-    bool wide = false;
+    uint32_t wide = 0;
     if (Q8) many_exps<D, Q8, TILE_THREADS>(S, pg.hole, key, s.len, ek, ev, wide);
     many_store<D, Q8, TILE_THREADS>(S, made, made + MANY_KEYS * D, bad, pg.hole, key, s.len, ek, ev);
     __syncthreads();
@@ -642,10 +652,12 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
                     }
                     ev_least = hi.ev < ev_least ? hi.ev : ev_least;
                     ev_most = hi.ev > ev_most ? hi.ev : ev_most;
-                    wide = wide || hi.wide;
                 }
+                if (Q8) wide = wide || ((hi.wide & 2) && masked);
                 float c = Q8 ? __builtin_amdgcn_ldexpf(cq, hi.ek) : cq;
                 c = fmaxf(c, 1e-37f);                        // -inf * c stays -inf at a scale of zero
+                // (a step of K's numbers, times D of q's, is below c / 8)
+                if (Q8 && (hi.wide & 1)) wide = wide || __any(c > 0x1p-8f);
                 float mx = ninf();
                 if (masked) {
                     // (the lane's half taken out first, so that what is compared with is constant:
@@ -710,8 +722,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 && NW == 4 ? 1 : 2) void k_kv_man
         }
         if (!g) asm volatile("s_barrier" ::: "memory");
         turn(c0(), cv(), n_tiles, []() {});
-        if (Q8 && (wide || ev_most - ev_least > 60)) {       // (of the whole block: its waves see the same tiles)
-            __syncthreads();
+        if (Q8 && __syncthreads_or(wide || ev_most - ev_least > 60)) {
             for (int i = 0; i < 32; i++) {
                 const int row = tile * ROWS + wave * 32 + i, j = row / group, r = s.r0 + j;
                 if (j >= nr || (unsigned)r >= (unsigned)b.n_rows) continue;
