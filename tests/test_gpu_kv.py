@@ -516,6 +516,55 @@ def test_append_and_read(pkg, fmt, dt, dim):
                 assert bool((o[p.n_rows:] == 77.0).all())
 
 
+@pytest.mark.parametrize("n_seq,most,hk,dim,page", [(64, 130, 4, 128, 64), (70, 131, 4, 64, 16), (90, 100, 3, 32, 32),
+                                                    (2100, 3, 5, 64, 16), (5000, 1, 3, 32, 16), (900, 12, 8, 128, 16)])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("fmt", ["q8", "bf16"])
+def test_append_and_read_many(pkg, fmt, dt, n_seq, most, hk, dim, page):
+    """Calls of many rows against the same rows in small calls, both ways, and
+    against the numbers that the format holds."""
+    say("append many", fmt, dt, n_seq, most, hk, dim, page)
+    r = np.random.default_rng(n_seq)
+    rows = r.integers(0, most + 1, n_seq)
+    rows[r.integers(n_seq)] = most
+    lens = rows + r.integers(0, 40, n_seq)
+    need = -(-lens // page)
+    n_pages = int(need.sum()) + 3
+    ids = r.permutation(n_pages).astype(np.int32)
+    table = np.full((n_seq, int(need.max())), -1, np.int32)
+    at = 0
+    for i in range(n_seq):
+        table[i, :need[i]] = ids[at:at + need[i]]
+        at += need[i]
+    row0 = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+    n = int(row0[-1])
+    t, kl, r0 = (torch.from_numpy(x.astype(np.int32)).to(DEV) for x in (table, lens, row0))
+    size = pkg.KvPool.page_bytes_of(fmt, page, hk, dim)
+    big = pkg.KvBatch(t, kl, r0, n, most, int(lens.max()))
+    small = [pkg.KvBatch(t[i:i + 50], kl[i:i + 50], r0[i:i + 51].clone(), n, most, int(lens.max())) for i in range(0, n_seq, 50)]
+    k, v = (torch.from_numpy(r.standard_normal((n, hk, dim)).astype(np.float32)).to(DT[dt]).to(DEV) for _ in range(2))
+    pools = []
+    for parts in ([big], small):
+        pool = pkg.KvPool(torch.full((n_pages, size), 0xFF, dtype=torch.uint8, device=DEV), fmt, page, hk, dim)
+        for b in parts:
+            pool.append(b, k, v)
+        pools.append(pool)
+    torch.cuda.synchronize()
+    assert torch.equal(pools[0].data, pools[1].data)
+    for parts in ([big], small):
+        ko, vo = (torch.full((n + 2, hk, dim), 77.0, device=DEV) for _ in range(2))
+        for b in parts:
+            pools[0].read(b, ko, vo)
+        torch.cuda.synchronize()
+        for x, o in ((k, ko), (v, vo)):
+            if fmt == "bf16":
+                want = x.to(torch.bfloat16).float()
+            else:
+                code, scale = quant(x.float().cpu().numpy())
+                want = torch.from_numpy((code.astype(np.float32) * scale[..., None]).reshape(n, hk, dim)).to(DEV)
+            assert torch.equal(o[:n], want) and bool((o[n:] == 77.0).all())
+
+
 def test_append_nonfinite(pkg):
     """NaN and infinities: a Q8 group with an infinity reads back as NaN, one
     with NaN as zeros (the sessions' rule), the other groups are untouched."""
