@@ -18,9 +18,12 @@ H = 2^-11 (of fp16), for a row with n keys, of width D:
 * the division and the output's rounding: 2 u of the result, B more for bf16.
 
 So with r = 2 ((D + 16) u + [bf16, q8] H) a + 2 (n + 64) u + [bf16] (2 B + H) the
-output is within 2 r sum_j p_j |v_j| + 2 n (2^-38 or 2^-25) max|v| p_max +
+output is within 2 r sum_j p_j |v_j| + 2 n (2^-38 or 2^-25) max|v| p_max (both
+over what the row attends) +
 ([bf16] B + 2 u) |o|: the weights enter the numerator and the denominator.
 """
+import threading
+
 import numpy as np
 import pytest
 
@@ -676,6 +679,38 @@ def test_streams_graphs_and_workspaces(pkg, lens):
         pool.append(p.batch, k, k)
         assert torch.equal(got, p.run(pool, q=q)) and torch.equal(got2, p2.run(pool2, q=q2))
     assert torch.equal(p2.run(pool2), eager2)
+
+
+def test_two_threads(pkg):
+    """Two host threads with a stream, outputs and a workspace each, on a
+    pool each: what each gets alone."""
+    say("two threads")
+    ps = [Problem(pkg, "q8", "bf16", 8, 2, 128, 64, lens, seed=2 + i, behind=0)
+          for i, lens in enumerate(([(4, 3000), (1, 200)], [(300, 2300), (5, 5)]))]
+    pools = [p.cache.pool() for p in ps]
+    alone = [p.run(pool) for p, pool in zip(ps, pools)]
+    ws = [p.ws(pool) for p, pool in zip(ps, pools)]
+    streams = [torch.cuda.Stream() for _ in ps]
+    outs = [[torch.full_like(p.q, 77.0) for _ in range(20)] for p in ps]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            for out in outs[i]:
+                pools[i].attend(ps[i].batch, ps[i].q, out, ps[i].scale, ws[i], stream=streams[i])
+        except Exception as e:                         # (a thread's own exception reaches nobody)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for i in range(2):
+        assert all(torch.equal(o, alone[i]) for o in outs[i])
 
 
 def test_same_bits_whatever_the_batch(pkg):
